@@ -315,6 +315,117 @@ int orc_attn_fused_at(const float* d_qkv, int ldqkv, int n_tok, int n_heads, int
                       int ctx, int pos_floor, int pos_limit, float* d_out, int ldo, void* d_work,
                       orc_stream_t stream);
 
+/* ── a cache in fewer bits, and several sequences over one prompt ────────────
+ * No reference counterpart (its cache is fp32 and holds one sequence). K and V
+ * are quantised as they are written and read as they are by the matrix cores;
+ * a batch of sequences may share the rows of a common prompt, which attention
+ * then reads once for all of them.
+ *
+ * A cache (one of K, one of V, for one layer) holds n_seq x n_kv x ctx rows of
+ * head_dim values, ctx a multiple of 64, head_dim 64 or 128, in
+ * orc_kvq_bytes() bytes of device memory (16-byte aligned, any contents at
+ * first). Its layout is the library's own: rows go in with orc_kvq_store and
+ * come out with orc_kvq_load; whole caches may be copied as bytes, and the
+ * bytes of one sequence are those of a cache of one sequence. Types:
+ *   ORC_F16     fp16 values; finite values beyond 65504 are stored as 65504
+ *               with their sign, infinities and NaN as they are;
+ *   ORC_KV_Q8   codes -127..127 and a scale per 32 head dims: the scale is the
+ *               smallest 8-bit float (5 exponent bits, 3 of the mantissa, bias
+ *               19: steps of 2^-21 up to 2^-18, then 3 bits) that reaches the
+ *               group's largest magnitude with code 127, a code the nearest
+ *               multiple, ties to even (an error of at most half a step, 1/225
+ *               of the group's largest value down to 2^-11, 2^-22 below);
+ *   ORC_KV_Q4   the same with codes -7..7 (half a step: at most 1/12.4).
+ * Q8 / Q4 values beyond 4064 are stored as 4064 with their sign; a group that
+ * holds an infinity or NaN reads back as NaN.
+ *
+ * Own positions: sequence i's rows are 0..ctx-1 of its part of the cache, and
+ * its new tokens are rows start_i, start_i + 1, ..., where start_i = d_pos[i] +
+ * pos_off (d_pos null: pos_off). A start outside the rows (a negative one
+ * marks an idle slot of a padded batch) stores nothing and attends to nothing,
+ * and so does a token behind the last row. */
+#define ORC_KV_Q8 259
+#define ORC_KV_Q4 260
+size_t orc_kvq_bytes(int type, int n_seq, int n_kv, int ctx, int head_dim); /* 0: no such cache */
+
+/* Rotary table of positions pos0 .. pos0 + n_pos - 1: [n_pos][rot_dim / 2]
+ * (cos, sin) pairs of pos * f_i, f_i = base^(-2 i / rot_dim), angles and
+ * functions in 64 bits, rounded once; rot_dim even, 2..128. `scaling` (null:
+ * none) stretches the frequencies for contexts beyond the trained one:
+ *   ORC_ROPE_LINEAR  f_i / factor;
+ *   ORC_ROPE_BANDS   by turns_i = orig_ctx f_i / (2 pi) over the original
+ *                    context: f_i above `high`, f_i / factor below `low`, in
+ *                    between the two mixed linearly in turns_i;
+ *   ORC_ROPE_YARN    mixed linearly in i, from f_i at the pair that makes
+ *                    `high` turns (rounded down, at least 0) to f_i / factor at
+ *                    the one that makes `low` (rounded up, at most rot_dim -
+ *                    1); the table's values times mscale (0: 0.1 ln(factor) +
+ *                    1).
+ * The table serves orc_kvq_store and, with rot_dim = head_dim and pos0 = 0,
+ * every other entry point that takes d_rope. */
+#define ORC_ROPE_PLAIN 0
+#define ORC_ROPE_LINEAR 1
+#define ORC_ROPE_BANDS 2
+#define ORC_ROPE_YARN 3
+typedef struct {
+    int kind;
+    float factor; /* >= 1 */
+    float low, high;
+    int orig_ctx;
+    float mscale;
+} orc_rope_scaling;
+int orc_rope_table(float* d_rope, int pos0, int n_pos, int rot_dim, double base, const orc_rope_scaling* scaling,
+                   orc_stream_t stream);
+
+/* The cache write of n_seq sequences of n_tok new tokens each (token t of
+ * sequence i is QKV row i n_tok + t, layout as orc_rope_kv_store): rotates the
+ * first rot_dim head dims of q and k (0: none; the rest stays as it is) by the
+ * pairs of position rope_off + own row in d_rope ([position][rot_dim / 2],
+ * which must reach rope_off + ctx), pairs (i, i + rot_dim / 2)
+ * (ORC_ROPE_HALF) or (2 i, 2 i + 1) (ORC_ROPE_PAIRS); writes the rotated q
+ * rows to d_q (which may be d_qkv, with ldq = ldqkv) and K and V, quantised,
+ * to the own rows. rope_off is the length of a shared prefix. Rotated values
+ * are exact sums rounded once to fp32. The K and V columns of the QKV rows are
+ * left as they are; so are q rows of tokens that are not stored, and every
+ * other row of the caches. Rows 16-byte aligned. */
+#define ORC_ROPE_HALF 0
+#define ORC_ROPE_PAIRS 1
+int orc_kvq_store(int type, const float* d_qkv, int ldqkv, int n_seq, int n_tok, int n_heads, int n_kv, int head_dim,
+                  int rope_layout, int rot_dim, const float* d_rope, int rope_off, const int32_t* d_pos, int pos_off,
+                  float* d_q, int ldq, void* d_kc, void* d_vc, int ctx, orc_stream_t stream);
+
+/* Rows start_i .. start_i + n - 1 of every sequence and kv head as fp32,
+ * [n_seq][n_kv][n][head_dim]: what the cache stands for, exactly. Rows outside
+ * the cache are zeros. K and V in one call; either pair (d_kc, d_k) or (d_vc,
+ * d_v) may be null. */
+int orc_kvq_load(int type, const void* d_kc, const void* d_vc, int n_seq, int n_kv, int head_dim, int ctx,
+                 const int32_t* d_pos, int pos_off, int n, float* d_k, float* d_v, orc_stream_t stream);
+
+/* Attention of n_seq sequences of n_tok new tokens over caches written by
+ * orc_kvq_store: query row i n_tok + t (ldq floats apart, rotated) attends to
+ * the prefix_len rows of the prefix caches d_pk / d_pv (one sequence's, of
+ * prefix_ctx rows; null with prefix_len 0) and to its own rows 0 .. start_i +
+ * t. Scale 1 / sqrt(head_dim), softmax with max subtraction, outputs in rows
+ * ldo floats apart. Any n_tok: a decode step, a verify pass, a prompt; any
+ * number of query heads per kv head. Tokens of an idle sequence, and tokens at
+ * or behind own row pos_limit (1..ctx), get zeros; the split of the work is
+ * sized by pos_limit, so a captured call serves every d_pos below it. With
+ * d_pos null, pos_off + n_tok must not exceed pos_limit.
+ * q is split in two fp16 halves (22 bits), the weights likewise, the cache's
+ * values are fp16 numbers: products are exact, sums fp32, and the error is
+ * that of an fp32 evaluation. Results depend on the shape of the call
+ * (n_seq, n_tok, prefix_len, pos_limit) in their rounding only. A NaN in a K or
+ * V row reaches the tokens that see the row; among the new tokens of one
+ * sequence a NaN or infinity in a V row may also reach the ones before it.
+ * Contents of rows that no token sees do not matter.
+ * d_work: orc_attn_kvq_workspace() bytes for the same arguments, 16-byte
+ * aligned (0 bytes: null); calls that share it must not overlap. */
+size_t orc_attn_kvq_workspace(int n_seq, int n_tok, int n_heads, int n_kv, int head_dim, int prefix_len, int pos_limit);
+int orc_attn_kvq(int type, const float* d_q, int ldq, int n_seq, int n_tok, int n_heads, int n_kv, int head_dim,
+                 const void* d_pk, const void* d_pv, int prefix_len, int prefix_ctx, const void* d_kc,
+                 const void* d_vc, int ctx, const int32_t* d_pos, int pos_off, int pos_limit, float* d_out, int ldo,
+                 void* d_work, orc_stream_t stream);
+
 /* ── argmax, sampling, acceptance ────────────────────────────────────────── */
 /* out[r] = first index of the maximum of row r (ops::argmax ops.cpp:490-497,
  * bench_engine.cpp:82-88). d_work needs orc_argmax_workspace() bytes. */

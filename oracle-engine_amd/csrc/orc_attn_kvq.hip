@@ -1,0 +1,582 @@
+// Attention over caches in fewer bits (gfx950): n_seq sequences of n_tok new
+// tokens over a prefix that all share and rows of their own (orc_attn_kvq).
+// The cache's layout and values: orc_kvq.hpp.
+//
+// Scores are formed transposed, S^T = K Q^T, so a lane holds one query row's
+// scores of 16 of a block's 64 keys, a row's softmax needs two exchanges
+// between lane groups for its maximum and none for the weights, and the
+// weights are already the second operand of O^T = V^T P^T. q and the weights are
+// two fp16 halves (22 bits), K and V fp16 numbers as stored: every product is
+// exact.
+// Sums: the matrix cores round toward minus infinity, so each block's products
+// start from zero and are added up in fp32 on the vector ALUs, and every other
+// block's weights are negated, so that what is left of that drift cancels.
+// The weights carry 2^15 (they cancel against their sum), which keeps both
+// halves normal fp16 numbers down to weights of 2^-29.
+#include "orc_kvq.hpp"
+
+#include <algorithm>
+#include <type_traits>
+
+namespace orc {
+
+constexpr int kKaWaves = 4;
+
+struct KaArgs {
+    const float* q;
+    int ldq, n_seq, n_tok, n_heads, n_kv, group;
+    const uint8_t *pk, *pv, *kc, *vc;
+    int prefix, pctx, ctx;
+    const int32_t* d_pos;
+    int pos_off, limit;
+    float* out;
+    int ldo;
+    float* part_o;   // [slot][row][hd], row = token n_heads + head
+    float2* part_ml; // [slot][row] (maximum, sum)
+    int n_rows;      // n_seq n_tok n_heads
+    // jobs: prefix ones (shared form only), then own ones
+    int shared, tiles_p, cp, tiles_o, co;
+};
+
+// Blocks [b0, b1) of chunk c of n chunks over nb blocks.
+__device__ __forceinline__ void ka_chunk(int nb, int n, int c, int& b0, int& b1) {
+    const int per = (nb + n - 1) / n;
+    b0 = min(nb, c * per);
+    b1 = min(nb, b0 + per);
+}
+
+// What a workgroup has to do: rows [r0, r1) of kv head `kv` (row = token G +
+// head in its group, tokens of all sequences in a row), key blocks [b0, b1) of
+// the prefix's nbp blocks and then the own ones of sequence seq.
+struct KaJob {
+    int kv, seq, r0, r1, b0, b1, slot, start, len;
+};
+
+__device__ __forceinline__ bool ka_job(const KaArgs& a, int m_rows, KaJob& j) {
+    // work items in order on each XCD: the row tiles of one chunk, which read the same keys, share its L2
+    const int jobs_p = a.shared ? a.n_kv * a.cp * a.tiles_p : 0, jobs = jobs_p + a.n_seq * a.n_kv * a.co * a.tiles_o;
+    const int per = (jobs + 7) / 8;
+    int w = (int)(blockIdx.x & 7) * per + (int)(blockIdx.x >> 3);
+    if (w >= jobs || (int)(blockIdx.x >> 3) >= per) return false;
+    const int nbp = (a.prefix + kKvBlock - 1) / kKvBlock;
+    if (w < jobs_p) {
+        const int tile = w % a.tiles_p, c = w / a.tiles_p % a.cp;
+        j.kv = w / a.tiles_p / a.cp;
+        j.seq = -1;
+        j.r0 = tile * m_rows;
+        j.r1 = min(j.r0 + m_rows, a.n_seq * a.n_tok * a.group);
+        j.start = j.len = 0;
+        j.slot = c;
+        ka_chunk(nbp, a.cp, c, j.b0, j.b1);
+        return true;
+    }
+    w -= jobs_p;
+    const int tile = a.tiles_o - 1 - w % a.tiles_o, c = w / a.tiles_o % a.co;  // the longest rows first
+    const int sk = w / a.tiles_o / a.co, rows = a.n_tok * a.group;
+    j.seq = sk / a.n_kv;
+    j.kv = sk % a.n_kv;
+    j.r0 = j.seq * rows + tile * m_rows;
+    j.r1 = min(j.r0 + m_rows, (j.seq + 1) * rows);
+    j.start = kvq_start(a.d_pos, j.seq, a.pos_off, a.limit);
+    j.len = j.start < 0 ? 0 : (int)min((int64_t)j.start + a.n_tok, (int64_t)a.limit);
+    j.slot = a.cp + c;
+    const int first = a.shared ? nbp : 0;
+    const int nb = j.len ? nbp - first + (j.len + kKvBlock - 1) / kKvBlock : 0;
+    ka_chunk(nb, a.co, c, j.b0, j.b1);
+    j.b0 += first;
+    j.b1 += first;
+    // nothing behind the tile's last token
+    const int last = min(j.start + (j.r1 - 1) / a.group - j.seq * a.n_tok, j.len - 1);
+    if (j.len) j.b1 = min(j.b1, nbp + last / kKvBlock + 1);
+    return true;
+}
+
+// ── operands ─────────────────────────────────────────────────────────────────
+// Bytes u of w (codes plus a bias) times their scales as fp16: 0x6400 | u is
+// 1024 + u.
+__device__ __forceinline__ void ka_cvt4(uint32_t w, kq_h2 s01, kq_h2 s23, _Float16 bias, kq_h2& o01, kq_h2& o23) {
+    const kq_h2 b = {bias, bias};
+    o01 = (__builtin_bit_cast(kq_h2, __builtin_amdgcn_perm(0x64646464u, w, 0x04010400u)) - b) * s01;
+    o23 = (__builtin_bit_cast(kq_h2, __builtin_amdgcn_perm(0x64646464u, w, 0x04030402u)) - b) * s23;
+}
+__device__ __forceinline__ kq_h8 ka_join(kq_h2 a, kq_h2 b, kq_h2 c, kq_h2 d) {
+    return kq_h8{a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
+}
+
+template <int TY> constexpr float ka_bias() { return 1024.f + kvq_levels(TY) + 1; }
+
+// One key tile's raw K bytes of a lane, and its operands.
+template <int TY, int HD> struct KaK {
+    static constexpr int kN = TY == ORC_F16 ? HD / 32 : TY == ORC_KV_Q8 ? HD / 64 : 1;
+    u32x4 r[kN];
+    __device__ __forceinline__ void load(const uint8_t* blk, int tile, int lane) {
+        const uint8_t* p = blk + tile * (16 * HD * kvq_bits(TY) / 8);
+        if constexpr (TY == ORC_KV_Q4 && HD == 64) {
+            const u32x2 v = *(const u32x2*)(p + lane * 8);
+            r[0].x = v.x;
+            r[0].y = v.y;
+        } else {
+#pragma unroll
+            for (int i = 0; i < kN; ++i) r[i] = *(const u32x4*)(p + i * 1024 + lane * 16);
+        }
+    }
+    // operand of dims j 8 .. j 8 + 7 of the lane; sc: the tile's scale twice
+    __device__ __forceinline__ kq_h8 op(int j, kq_h2 sc) const {
+        if constexpr (TY == ORC_F16) return __builtin_bit_cast(kq_h8, r[j]);
+        else {
+            uint32_t w0, w1;
+            if constexpr (TY == ORC_KV_Q8) {
+                w0 = r[j / 2][(j & 1) * 2];
+                w1 = r[j / 2][(j & 1) * 2 + 1];
+            } else {
+                constexpr int half = HD / 64;  // steps in the low halves
+                const int i = j % half * 2, sh = j / half * 4;
+                w0 = (r[0][i] >> sh) & 0x0F0F0F0Fu;
+                w1 = (r[0][i + 1] >> sh) & 0x0F0F0F0Fu;
+            }
+            kq_h2 o[4];
+            ka_cvt4(w0, sc, sc, (_Float16)ka_bias<TY>(), o[0], o[1]);
+            ka_cvt4(w1, sc, sc, (_Float16)ka_bias<TY>(), o[2], o[3]);
+            return ka_join(o[0], o[1], o[2], o[3]);
+        }
+    }
+};
+
+// Scale of tile T from the dword of the lane's key and group.
+__device__ __forceinline__ kq_h2 ka_scale_k(uint32_t w, int T) {
+    return __builtin_bit_cast(kq_h2, __builtin_amdgcn_perm(0u, w, 0x000C000Cu | (T << 8) | (T << 24)) >> 1);
+}
+// Scales of bytes e, e + 1 of w.
+__device__ __forceinline__ kq_h2 ka_scale_v(uint32_t w, int e) {
+    return __builtin_bit_cast(kq_h2, __builtin_amdgcn_perm(0u, w, 0x000C000Cu | (e << 8) | ((e + 1) << 24)) >> 1);
+}
+
+// V bytes of one dim tile (both tiles of a pair for 4 bits) of a lane.
+template <int TY, int HD> struct KaV {
+    static constexpr int kN = TY == ORC_F16 ? HD / 8 : TY == ORC_KV_Q8 ? HD / 16 : HD / 32;
+    u32x4 r[kN];
+    u32x4 sc[TY == ORC_F16 ? 1 : HD / 32];
+    __device__ __forceinline__ void load(const uint8_t* blk, int lane) {
+#pragma unroll
+        for (int i = 0; i < kN; ++i) r[i] = *(const u32x4*)(blk + i * 1024 + lane * 16);
+        if constexpr (TY != ORC_F16) {
+#pragma unroll
+            for (int i = 0; i < HD / 32; ++i)
+                sc[i] = *(const u32x4*)(blk + kvq_code_bytes(TY, HD) + i * 64 + (lane >> 4) * 16);
+        }
+    }
+    // The rows from key `n` of the block on count as zeros (0 times whatever they hold would not): the bytes'
+    // scales, or the halves themselves.
+    __device__ __forceinline__ void keep(int n, int lane) {
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+                const int k = min(max(n - (s * 32 + q * 16 + (lane >> 4) * 4), 0), 4);
+                if constexpr (TY == ORC_F16) {
+                    const uint32_t m0 = k >= 2 ? ~0u : k ? 0xFFFFu : 0u, m1 = k >= 4 ? ~0u : k == 3 ? 0xFFFFu : 0u;
+#pragma unroll
+                    for (int dt = 0; dt < HD / 16; ++dt) {
+                        r[dt * 2 + s][q * 2] &= m0;
+                        r[dt * 2 + s][q * 2 + 1] &= m1;
+                    }
+                } else {
+                    const uint32_t m = k >= 4 ? ~0u : (1u << (8 * k)) - 1u;
+#pragma unroll
+                    for (int g = 0; g < HD / 32; ++g) sc[g][s * 2 + q] &= m;
+                }
+            }
+    }
+    // operand of dim tile dt and the 32 keys of step s
+    __device__ __forceinline__ kq_h8 op(int dt, int s) const {
+        if constexpr (TY == ORC_F16) return __builtin_bit_cast(kq_h8, r[dt * 2 + s]);
+        else {
+            uint32_t w0, w1;
+            if constexpr (TY == ORC_KV_Q8) {
+                w0 = r[dt][s * 2];
+                w1 = r[dt][s * 2 + 1];
+            } else {
+                w0 = (r[dt / 2][s * 2] >> (dt & 1) * 4) & 0x0F0F0F0Fu;
+                w1 = (r[dt / 2][s * 2 + 1] >> (dt & 1) * 4) & 0x0F0F0F0Fu;
+            }
+            const uint32_t s0 = sc[dt / 2][s * 2], s1 = sc[dt / 2][s * 2 + 1];
+            kq_h2 o[4];
+            ka_cvt4(w0, ka_scale_v(s0, 0), ka_scale_v(s0, 2), (_Float16)ka_bias<TY>(), o[0], o[1]);
+            ka_cvt4(w1, ka_scale_v(s1, 0), ka_scale_v(s1, 2), (_Float16)ka_bias<TY>(), o[2], o[3]);
+            return ka_join(o[0], o[1], o[2], o[3]);
+        }
+    }
+};
+
+// Two fp16 halves of a and b.
+__device__ __forceinline__ uint32_t ka_split(float a, float b, uint32_t& lo) {
+    const kq_h2 hi = __builtin_bit_cast(kq_h2, __builtin_amdgcn_cvt_pkrtz(a, b));
+    lo = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(a - (float)hi.x, b - (float)hi.y));
+    return __builtin_bit_cast(uint32_t, hi);
+}
+
+// A query row as operands: its head dims (hd / 4 per lane group) times a power
+// of two that brings the largest below 2^15, in two halves; f turns its scores into powers of two.
+template <int TY, int HD> struct KaQ {
+    kq_h8 hi[HD / 32], lo[HD / 32];
+    float f;
+    __device__ __forceinline__ void load(const float* p, bool live, int g) {
+        float v[HD / 4];
+        float mx = 0.f;
+#pragma unroll
+        for (int i = 0; i < HD / 16; ++i) {
+            kq_f4 t = {0.f, 0.f, 0.f, 0.f};
+            if (live) t = *(const kq_f4*)(p + g * (HD / 4) + i * 4);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                v[i * 4 + e] = t[e];
+                mx = fmaxf(mx, fabsf(t[e]));
+            }
+        }
+        mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+        mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+        int ex = 0;
+        if (mx > 0.f && mx < __builtin_inff()) (void)frexpf(mx, &ex);
+        ex = max(-96, min(15 - ex, 120));
+        f = ldexpf(1.4426950408889634f / (HD == 64 ? 8.f : 11.313708498984761f) * (TY == ORC_F16 ? 1.f : 0.0625f), -ex);
+#pragma unroll
+        for (int j = 0; j < HD / 32; ++j) {
+            uint32_t h[4], l[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                h[e] = ka_split(ldexpf(v[j * 8 + 2 * e], ex), ldexpf(v[j * 8 + 2 * e + 1], ex), l[e]);
+            hi[j] = __builtin_bit_cast(kq_h8, u32x4{h[0], h[1], h[2], h[3]});
+            lo[j] = __builtin_bit_cast(kq_h8, u32x4{l[0], l[1], l[2], l[3]});
+        }
+    }
+};
+
+__device__ __forceinline__ kq_f4 ka_mfma(kq_h8 a, kq_h8 b, kq_f4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+
+// Running softmax of one row (per lane; the four lanes of a row agree on m,
+// each sums its own keys).
+struct KaRow {
+    float m = -__builtin_inff(), l = 0.f;
+    // scores s of the lane's 16 keys -> weights times 2^15 and sign; returns what the sums so far are scaled by
+    __device__ __forceinline__ float step(kq_f4 (&s)[4], float f, uint32_t sign, u32x4 (&hi)[2], u32x4 (&lo)[2]) {
+        float mx = fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3]));
+#pragma unroll
+        for (int t = 1; t < 4; ++t) mx = fmaxf(fmaxf(mx, fmaxf(s[t][0], s[t][1])), fmaxf(s[t][2], s[t][3]));
+        mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+        mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+        const float mn = fmaxf(m, mx * f), ref = mn == -__builtin_inff() ? 0.f : mn;
+        const float alpha = __builtin_amdgcn_exp2f(m - ref);
+        m = mn;
+        float sum = 0.f;
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+            float p[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                p[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][i], f, 15.f - ref));
+                sum += p[i];
+            }
+            uint32_t l0, l1;
+            const uint32_t h0 = ka_split(p[0], p[1], l0), h1 = ka_split(p[2], p[3], l1);
+            hi[t / 2][(t & 1) * 2] = h0 ^ sign;
+            hi[t / 2][(t & 1) * 2 + 1] = h1 ^ sign;
+            lo[t / 2][(t & 1) * 2] = l0 ^ sign;
+            lo[t / 2][(t & 1) * 2 + 1] = l1 ^ sign;
+        }
+        l = l * alpha + sum;
+        return alpha;
+    }
+};
+
+// ── few rows: the waves share out the keys ───────────────────────────────────
+// A workgroup takes 16 RT rows; its waves take every fourth key block each,
+// straight from memory to operands, and join their sums at the end.
+template <int TY, int HD, int RT> __global__ __launch_bounds__(64 * kKaWaves) void k_attn_kvq(KaArgs a) {
+    constexpr int DT = HD / 16, KS = HD / 32, BB = kvq_block_bytes(TY, HD), M = 16 * RT;
+    __shared__ float sh_o[kKaWaves][M][HD + 4];
+    __shared__ float2 sh_ml[kKaWaves][M];
+    KaJob j;
+    if (!ka_job(a, M, j)) return;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = lane & 15, g = lane >> 4;
+    const bool direct = a.cp + a.co == 1;
+    if (j.b0 >= j.b1 && !direct) return;
+    const int nbp = (a.prefix + kKvBlock - 1) / kKvBlock;
+
+    KaQ<TY, HD> q[RT];
+    KaRow st[RT];
+    int vis[RT];  // own rows that the lane's query row sees
+    kq_f4 o[RT][DT];
+#pragma unroll
+    for (int r = 0; r < RT; ++r) {
+        const int row = j.r0 + r * 16 + c, tok = row / a.group, hg = row - tok * a.group;
+        q[r].load(a.q + (int64_t)tok * a.ldq + (size_t)(j.kv * a.group + hg) * HD, row < j.r1, g);
+        vis[r] = j.seq < 0 ? 0 : min(j.start + tok - j.seq * a.n_tok + 1, j.len);
+#pragma unroll
+        for (int d = 0; d < DT; ++d) o[r][d] = kq_f4{0.f, 0.f, 0.f, 0.f};
+    }
+    const int first_own = j.seq < 0 ? 0 : min(j.start + j.r0 / a.group - j.seq * a.n_tok + 1, j.len);  // the least vis
+    const uint8_t* pk = a.pk + (size_t)j.kv * (a.pctx / kKvBlock) * BB;
+    const uint8_t* pv = a.pv + (size_t)j.kv * (a.pctx / kKvBlock) * BB;
+    const size_t own = ((size_t)max(j.seq, 0) * a.n_kv + j.kv) * (a.ctx / kKvBlock) * BB;
+    float sgn = 1.f;
+    for (int b = j.b0 + wave; b < j.b1; b += kKaWaves) {
+        const bool pre = b < nbp;
+        const uint8_t* kb = pre ? pk + (size_t)b * BB : a.kc + own + (size_t)(b - nbp) * BB;
+        const uint8_t* vb = pre ? pv + (size_t)b * BB : a.vc + own + (size_t)(b - nbp) * BB;
+        KaK<TY, HD> kr[4];
+        KaV<TY, HD> vr;
+        uint32_t ks = 0;
+#pragma unroll
+        for (int t = 0; t < 4; ++t) kr[t].load(kb, t, lane);
+        if constexpr (TY != ORC_F16) ks = *(const uint32_t*)(kb + kvq_code_bytes(TY, HD) + ((HD == 128 ? g : g >> 1) * 16 + c) * 4);
+        vr.load(vb, lane);
+        const int key0 = (pre ? b : b - nbp) * kKvBlock, lim = (pre ? a.prefix : j.len) - key0;
+        kq_f4 s[RT][4];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+            kq_h2 sc = {};
+            if constexpr (TY != ORC_F16) sc = ka_scale_k(ks, t);
+            kq_h8 k[KS];
+#pragma unroll
+            for (int i = 0; i < KS; ++i) k[i] = kr[t].op(i, sc);
+#pragma unroll
+            for (int r = 0; r < RT; ++r) {
+                kq_f4 z = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int i = 0; i < KS; ++i) z = ka_mfma(k[i], q[r].lo[i], z);
+#pragma unroll
+                for (int i = 0; i < KS; ++i) z = ka_mfma(k[i], q[r].hi[i], z);
+                s[r][t] = z;
+            }
+        }
+        if (lim < kKvBlock || (!pre && first_own - key0 < kKvBlock)) {
+#pragma unroll
+            for (int r = 0; r < RT; ++r) {
+                const int n = pre ? lim : min(lim, vis[r] - key0);
+#pragma unroll
+                for (int t = 0; t < 4; ++t)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (t * 16 + g * 4 + i >= n) s[r][t][i] = -__builtin_inff();
+            }
+        }
+        if (lim < kKvBlock) vr.keep(lim, lane);
+        sgn = -sgn;
+        const uint32_t sign = sgn < 0.f ? 0x80008000u : 0u;
+        u32x4 ph[RT][2], pl[RT][2];
+        float beta[RT];
+#pragma unroll
+        for (int r = 0; r < RT; ++r) beta[r] = -st[r].step(s[r], q[r].f, sign, ph[r], pl[r]);
+#pragma unroll
+        for (int d = 0; d < DT; ++d) {
+            const kq_h8 v0 = vr.op(d, 0), v1 = vr.op(d, 1);
+#pragma unroll
+            for (int r = 0; r < RT; ++r) {
+                kq_f4 z = {0.f, 0.f, 0.f, 0.f};
+                z = ka_mfma(v0, __builtin_bit_cast(kq_h8, pl[r][0]), z);
+                z = ka_mfma(v1, __builtin_bit_cast(kq_h8, pl[r][1]), z);
+                z = ka_mfma(v0, __builtin_bit_cast(kq_h8, ph[r][0]), z);
+                z = ka_mfma(v1, __builtin_bit_cast(kq_h8, ph[r][1]), z);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) o[r][d][i] = __builtin_fmaf(o[r][d][i], beta[r], z[i]);
+            }
+        }
+    }
+    // join the waves' sums
+#pragma unroll
+    for (int r = 0; r < RT; ++r) {
+        float l = st[r].l;
+        l += __shfl_xor(l, 16, 64);
+        l += __shfl_xor(l, 32, 64);
+        st[r].l = l;
+        if (g == 0) sh_ml[wave][r * 16 + c] = make_float2(st[r].m, l);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < RT; ++r) {
+        float mm = sh_ml[0][r * 16 + c].x;
+#pragma unroll
+        for (int w = 1; w < kKaWaves; ++w) mm = fmaxf(mm, sh_ml[w][r * 16 + c].x);
+        const float e = st[r].l == 0.f ? 0.f : __builtin_amdgcn_exp2f(st[r].m - mm) * sgn;
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                sh_o[wave][r * 16 + c][d * 16 + g * 4 + i] = st[r].l == 0.f ? 0.f : o[r][d][i] * e;
+    }
+    __syncthreads();
+    for (int it = tid; it < M * (HD / 4); it += 64 * kKaWaves) {
+        const int rr = it / (HD / 4), d = it % (HD / 4) * 4, row = j.r0 + rr;
+        if (row >= j.r1) continue;
+        float mm = sh_ml[0][rr].x, l = 0.f;
+#pragma unroll
+        for (int w = 1; w < kKaWaves; ++w) mm = fmaxf(mm, sh_ml[w][rr].x);
+        kq_f4 v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int w = 0; w < kKaWaves; ++w) {
+            const float2 ml = sh_ml[w][rr];
+            if (ml.y != 0.f) l += ml.y * __builtin_amdgcn_exp2f(ml.x - mm);
+            v += *(const kq_f4*)&sh_o[w][rr][d];
+        }
+        const int tok = row / a.group, head = j.kv * a.group + (row - tok * a.group);
+        if (direct) {
+            const bool live = j.start >= 0 && j.start + (int64_t)(tok - j.seq * a.n_tok) < a.limit;
+            const float inv = (TY == ORC_F16 ? 1.f : 0.0625f) / l;
+            kq_f4 y = {0.f, 0.f, 0.f, 0.f};
+            if (live && l != 0.f) y = v * inv;
+            *(kq_f4*)(a.out + (int64_t)tok * a.ldo + (size_t)head * HD + d) = y;
+        } else {
+            const size_t at = (size_t)j.slot * a.n_rows + (size_t)tok * a.n_heads + head;
+            *(kq_f4*)(a.part_o + at * HD + d) = v;
+            if (d == 0) a.part_ml[at] = make_float2(mm, l);
+        }
+    }
+}
+
+// ── the chunks' partial sums ─────────────────────────────────────────────────
+// One wave per row: out = sum over chunks of 2^(m_c - max) O_c over the same of l_c.
+template <int HD> __global__ __launch_bounds__(256) void k_attn_kvq_merge(KaArgs a, float unit) {
+    const int lane = threadIdx.x & 63;
+    const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (row >= a.n_rows) return;
+    constexpr int E = HD / 64;
+    const int tok = (int)(row / a.n_heads), head = (int)(row - (int64_t)tok * a.n_heads), seq = tok / a.n_tok;
+    const int start = kvq_start(a.d_pos, seq, a.pos_off, a.limit);
+    float* out = a.out + (int64_t)tok * a.ldo + (size_t)head * HD;
+    float v[E] = {};
+    float l = 0.f;
+    if (start >= 0 && start + (int64_t)(tok - seq * a.n_tok) < a.limit) {
+        const int len = (int)min((int64_t)start + a.n_tok, (int64_t)a.limit);
+        const int nbp = (a.prefix + kKvBlock - 1) / kKvBlock, first = a.shared ? nbp : 0;
+        const int nb = nbp - first + (len + kKvBlock - 1) / kKvBlock;
+        const int last = nbp - first + (start + tok - seq * a.n_tok) / kKvBlock;  // the row's last block
+        float m = -__builtin_inff();
+        for (int pass = 0; pass < 2; ++pass)
+            for (int c = 0; c < a.cp + a.co; ++c) {
+                int b0, b1;
+                if (c < a.cp) ka_chunk(nbp, a.cp, c, b0, b1);
+                else ka_chunk(nb, a.co, c - a.cp, b0, b1);
+                if (b0 >= b1 || (c >= a.cp && b0 > last)) continue;
+                const size_t at = (size_t)c * a.n_rows + row;
+                const float2 ml = a.part_ml[at];
+                if (pass == 0) {
+                    m = fmaxf(m, ml.x);
+                    continue;
+                }
+                if (ml.y == 0.f) continue;
+                const float e = __builtin_amdgcn_exp2f(ml.x - m);
+                l += e * ml.y;
+#pragma unroll
+                for (int i = 0; i < E; ++i) v[i] += e * a.part_o[at * HD + lane + 64 * i];
+            }
+    }
+#pragma unroll
+    for (int i = 0; i < E; ++i) out[lane + 64 * i] = l == 0.f ? 0.f : v[i] * (unit / l);
+}
+
+// ── host ─────────────────────────────────────────────────────────────────────
+struct KaPlan {
+    bool shared;
+    int rt_p, rt_o, tiles_p, cp, tiles_o, co;
+    size_t rows;
+    int slots() const { return cp + co; }
+    size_t bytes(int hd) const { return slots() > 1 ? (size_t)slots() * rows * (4 * (size_t)hd + 8) : 0; }
+};
+
+static int ka_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
+
+// Chunks of nb key blocks for `base` workgroups' worth of row tiles: about two
+// workgroups per CU, and a block for every wave.
+static int ka_chunks(int64_t base, int nb) {
+    return (int)std::max<int64_t>(1, std::min<int64_t>((512 + base - 1) / base, nb / kKaWaves));
+}
+
+static KaPlan ka_plan(int n_seq, int n_tok, int n_heads, int n_kv, int prefix_len, int pos_limit) {
+    KaPlan p{};
+    const int64_t group = n_heads / n_kv, rows_o = n_tok * group, rows_p = n_seq * rows_o;
+    p.rows = (size_t)n_seq * n_tok * n_heads;
+    const int nbp = ka_div(prefix_len, kKvBlock), nbo = ka_div(pos_limit, kKvBlock);
+    p.shared = prefix_len > 0 && n_seq > 1;
+    p.rt_o = p.rt_p = (p.shared ? rows_p : rows_o) > 16 ? 2 : 1;
+    p.tiles_o = ka_div(rows_o, 16 * p.rt_o);
+    p.co = ka_chunks((int64_t)n_seq * n_kv * p.tiles_o, p.shared ? nbo : nbp + nbo);
+    if (p.shared) {
+        p.tiles_p = ka_div(rows_p, 16 * p.rt_p);
+        p.cp = ka_chunks((int64_t)n_kv * p.tiles_p, nbp);
+    }
+    return p;
+}
+
+template <int TY, int HD> static void ka_launch(const KaPlan& p, const KaArgs& a, hipStream_t s) {
+    const int64_t jobs = (int64_t)a.n_kv * p.cp * p.tiles_p + (int64_t)a.n_seq * a.n_kv * p.co * p.tiles_o;
+    const dim3 grid((unsigned)((jobs + 7) / 8 * 8));
+    if (p.rt_o == 1) hipLaunchKernelGGL((k_attn_kvq<TY, HD, 1>), grid, dim3(64 * kKaWaves), 0, s, a);
+    else hipLaunchKernelGGL((k_attn_kvq<TY, HD, 2>), grid, dim3(64 * kKaWaves), 0, s, a);
+}
+
+}  // namespace orc
+
+using namespace orc;
+
+static bool ka_shape_ok(int n_seq, int n_tok, int n_heads, int n_kv, int prefix_len, int pos_limit) {
+    return n_seq >= 1 && n_tok >= 1 && n_heads >= 1 && n_kv >= 1 && n_heads % n_kv == 0 && prefix_len >= 0 && pos_limit >= 1 &&
+           (int64_t)n_seq * n_tok <= 0x7fffffff / n_heads && (int64_t)prefix_len + pos_limit + n_tok <= 0x7fffff00;
+}
+
+extern "C" size_t orc_attn_kvq_workspace(int n_seq, int n_tok, int n_heads, int n_kv, int head_dim, int prefix_len,
+                                         int pos_limit) {
+    if ((head_dim != 64 && head_dim != 128) || !ka_shape_ok(n_seq, n_tok, n_heads, n_kv, prefix_len, pos_limit)) return 0;
+    return ka_plan(n_seq, n_tok, n_heads, n_kv, prefix_len, pos_limit).bytes(head_dim);
+}
+
+extern "C" int orc_attn_kvq(int type, const float* d_q, int ldq, int n_seq, int n_tok, int n_heads, int n_kv,
+                            int head_dim, const void* d_pk, const void* d_pv, int prefix_len, int prefix_ctx,
+                            const void* d_kc, const void* d_vc, int ctx, const int32_t* d_pos, int pos_off,
+                            int pos_limit, float* d_out, int ldo, void* d_work, orc_stream_t s) {
+    if (!initialized()) return set_error(ORC_E_NOINIT, "orc_init not called");
+    if (!kvq_type_ok(type)) return set_error(ORC_E_UNSUPPORTED, "attn_kvq: cache types are F16, KV_Q8 and KV_Q4");
+    if (head_dim != 64 && head_dim != 128) return set_error(ORC_E_UNSUPPORTED, "attn_kvq: head_dim must be 64 or 128");
+    if (n_seq < 0 || n_tok < 0) return set_error(ORC_E_INVALID, "attn_kvq: bad args");
+    if (!n_seq || !n_tok) return ORC_OK;
+    if (!ka_shape_ok(n_seq, n_tok, n_heads, n_kv, prefix_len, pos_limit) || ctx % kKvBlock || pos_limit > ctx ||
+        prefix_len > prefix_ctx || prefix_ctx % kKvBlock || ldq < (int64_t)n_heads * head_dim ||
+        ldo < (int64_t)n_heads * head_dim || ldq % 4 || ldo % 4)
+        return set_error(ORC_E_INVALID, "attn_kvq: bad args (heads a multiple of the kv heads, 1 <= pos_limit <= ctx, "
+                                        "prefix_len <= prefix_ctx, contexts multiples of 64)");
+    if (!d_pos && (pos_off < 0 || (int64_t)pos_off + n_tok > pos_limit))
+        return set_error(ORC_E_INVALID, "attn_kvq: positions must lie below pos_limit");
+    const KaPlan p = ka_plan(n_seq, n_tok, n_heads, n_kv, prefix_len, pos_limit);
+    const size_t bytes = p.bytes(head_dim);
+    if (!d_q || !d_out || !d_kc || !d_vc || (prefix_len && (!d_pk || !d_pv)) || (bytes && !d_work) ||
+        (((uintptr_t)d_q | (uintptr_t)d_out | (uintptr_t)d_kc | (uintptr_t)d_vc | (uintptr_t)d_pk | (uintptr_t)d_pv |
+          (uintptr_t)d_work) & 15))
+        return set_error(ORC_E_INVALID, "attn_kvq: null or misaligned pointer");
+    const int64_t jobs = (int64_t)n_kv * p.cp * p.tiles_p + (int64_t)n_seq * n_kv * p.co * p.tiles_o;
+    if (jobs > 0xffffff00ll / 256 - 8) return set_error(ORC_E_INVALID, "attn_kvq: too many rows");
+    KaArgs a{d_q, ldq, n_seq, n_tok, n_heads, n_kv, n_heads / n_kv, (const uint8_t*)d_pk, (const uint8_t*)d_pv,
+             (const uint8_t*)d_kc, (const uint8_t*)d_vc, prefix_len, prefix_ctx, ctx, d_pos, pos_off, pos_limit, d_out,
+             ldo, nullptr, nullptr, (int)p.rows, p.shared, p.tiles_p, p.cp, p.tiles_o, p.co};
+    if (bytes) {
+        a.part_o = (float*)d_work;
+        a.part_ml = (float2*)((uint8_t*)d_work + (size_t)p.slots() * p.rows * head_dim * 4);
+    }
+    const hipStream_t st = resolve_stream(s);
+    auto go = [&](auto ty) {
+        constexpr int T = decltype(ty)::value;
+        head_dim == 64 ? ka_launch<T, 64>(p, a, st) : ka_launch<T, 128>(p, a, st);
+    };
+    if (type == ORC_F16) go(std::integral_constant<int, ORC_F16>());
+    else if (type == ORC_KV_Q8) go(std::integral_constant<int, ORC_KV_Q8>());
+    else go(std::integral_constant<int, ORC_KV_Q4>());
+    ORC_LAUNCH_CHECK();
+    if (p.slots() > 1) {
+        const dim3 grid((unsigned)ka_div((int64_t)p.rows, 4));
+        const float unit = type == ORC_F16 ? 1.f : 0.0625f;
+        if (head_dim == 64) hipLaunchKernelGGL(k_attn_kvq_merge<64>, grid, dim3(256), 0, st, a, unit);
+        else hipLaunchKernelGGL(k_attn_kvq_merge<128>, grid, dim3(256), 0, st, a, unit);
+        ORC_LAUNCH_CHECK();
+    }
+    return ORC_OK;
+}

@@ -18,6 +18,9 @@ BIN_DIR = os.path.join(PKG, "bin")
 F32, F16, Q4_0, Q8_0, Q4_K, Q6_K = 0, 1, 2, 8, 12, 14
 EPI_STORE, EPI_ACCUM, EPI_SWIGLU = 0, 1, 2
 Q8_0_X8 = 258  # ORC_Q8_0_X8: Q8_0 regrouped by orc_q8_0_regroup
+KV_Q8, KV_Q4 = 259, 260  # cache types of orc_kvq_store (and F16)
+ROPE_PLAIN, ROPE_LINEAR, ROPE_BANDS, ROPE_YARN = 0, 1, 2, 3
+ROPE_HALF, ROPE_PAIRS = 0, 1
 
 _vp = C.c_void_p
 _fp = C.POINTER(C.c_float)
@@ -30,6 +33,11 @@ class OrcError(RuntimeError):
 
 class Seg(C.Structure):
     _fields_ = [("d_w", _vp), ("n_out", C.c_int), ("d_y", _vp), ("d_bias", _vp)]
+
+
+class RopeScaling(C.Structure):
+    _fields_ = [("kind", C.c_int), ("factor", C.c_float), ("low", C.c_float), ("high", C.c_float),
+                ("orig_ctx", C.c_int), ("mscale", C.c_float)]
 
 
 # (name, restype, argtypes) for every entry point declared in include/orc.h
@@ -83,6 +91,15 @@ ABI = [
                                    _vp, C.c_int, _vp]),
     ("orc_attn_fused_at", C.c_int, [_vp, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, _vp, C.c_int, _vp, _vp, _vp,
                                     C.c_int, C.c_int, C.c_int, _vp, C.c_int, _vp, _vp]),
+    ("orc_kvq_bytes", C.c_size_t, [C.c_int] * 5),
+    ("orc_rope_table", C.c_int, [_vp, C.c_int, C.c_int, C.c_int, C.c_double, C.POINTER(RopeScaling), _vp]),
+    ("orc_kvq_store", C.c_int, [C.c_int, _vp, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int,
+                                _vp, C.c_int, _vp, C.c_int, _vp, C.c_int, _vp, _vp, C.c_int, _vp]),
+    ("orc_kvq_load", C.c_int, [C.c_int, _vp, _vp, C.c_int, C.c_int, C.c_int, C.c_int, _vp, C.c_int, C.c_int, _vp, _vp,
+                               _vp]),
+    ("orc_attn_kvq_workspace", C.c_size_t, [C.c_int] * 7),
+    ("orc_attn_kvq", C.c_int, [C.c_int, _vp, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, _vp, _vp, C.c_int,
+                               C.c_int, _vp, _vp, C.c_int, _vp, C.c_int, C.c_int, _vp, C.c_int, _vp, _vp]),
     ("orc_argmax_workspace", C.c_size_t, [C.c_int, C.c_int]),
     ("orc_argmax", C.c_int, [_vp, C.c_int, C.c_int, C.c_int, _vp, _vp, _vp]),
     ("orc_argmax_noalloc", C.c_int, [_vp, C.c_int, C.c_int, C.c_int, _vp, _vp]),
