@@ -34,8 +34,9 @@ struct KaArgs {
     float* part_o;   // [slot][row][hd], row = token n_heads + head
     float2* part_ml; // [slot][row] (maximum, sum)
     int n_rows;      // n_seq n_tok n_heads
-    // jobs: prefix ones (shared form only), then own ones
+    // jobs: prefix ones (shared form only), then own ones; a launch takes `jobs` of them from `job0` on
     int shared, tiles_p, cp, tiles_o, co;
+    int job0, jobs;
 };
 
 // Blocks [b0, b1) of chunk c of n chunks over nb blocks.
@@ -54,10 +55,10 @@ struct KaJob {
 
 __device__ __forceinline__ bool ka_job(const KaArgs& a, int m_rows, KaJob& j) {
     // work items in order on each XCD: the row tiles of one chunk, which read the same keys, share its L2
-    const int jobs_p = a.shared ? a.n_kv * a.cp * a.tiles_p : 0, jobs = jobs_p + a.n_seq * a.n_kv * a.co * a.tiles_o;
-    const int per = (jobs + 7) / 8;
+    const int jobs_p = a.shared ? a.n_kv * a.cp * a.tiles_p : 0, per = (a.jobs + 7) / 8;
     int w = (int)(blockIdx.x & 7) * per + (int)(blockIdx.x >> 3);
-    if (w >= jobs || (int)(blockIdx.x >> 3) >= per) return false;
+    if (w >= a.jobs) return false;
+    w += a.job0;
     const int nbp = (a.prefix + kKvBlock - 1) / kKvBlock;
     if (w < jobs_p) {
         const int tile = w % a.tiles_p, c = w / a.tiles_p % a.cp;
@@ -435,51 +436,296 @@ template <int TY, int HD, int RT> __global__ __launch_bounds__(64 * kKaWaves) vo
     }
 }
 
+// ── many rows: the waves share the keys' operands ────────────────────────────
+// A workgroup takes 64 RT rows, 16 RT a wave, through every key block of its
+// chunk. Each wave turns a quarter of the block into operands in LDS (two
+// buffers, one barrier per block), the next block's bytes are on their way
+// meanwhile: the conversion costs a quarter of what it would in each wave, and
+// an operand read serves 2 RT products.
+template <int TY, int HD> struct KaStage {
+    static constexpr int DW = HD / 64;  // dim tiles of V a wave stages
+    KaK<TY, HD> k;
+    uint32_t ks;
+    u32x4 v[TY == ORC_F16 ? DW * 2 : TY == ORC_KV_Q8 ? DW : 1], vs;
+    __device__ __forceinline__ void load(const uint8_t* kb, const uint8_t* vb, int wave, int lane) {
+        const int c = lane & 15, g = lane >> 4;
+        k.load(kb, wave, lane);
+        if constexpr (TY == ORC_F16) {
+#pragma unroll
+            for (int i = 0; i < DW * 2; ++i) v[i] = *(const u32x4*)(vb + (wave * DW * 2 + i) * 1024 + lane * 16);
+        } else {
+            ks = *(const uint32_t*)(kb + kvq_code_bytes(TY, HD) + ((HD == 128 ? g : g >> 1) * 16 + c) * 4);
+            vs = *(const u32x4*)(vb + kvq_code_bytes(TY, HD) + (wave * DW >> 1) * 64 + g * 16);
+            if constexpr (TY == ORC_KV_Q8) {
+#pragma unroll
+                for (int i = 0; i < DW; ++i) v[i] = *(const u32x4*)(vb + (wave * DW + i) * 1024 + lane * 16);
+            } else
+                v[0] = *(const u32x4*)(vb + (wave * DW >> 1) * 1024 + lane * 16);
+        }
+    }
+    __device__ __forceinline__ void keep(int n, int lane) {
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+                const int m = min(max(n - (s * 32 + q * 16 + (lane >> 4) * 4), 0), 4);
+                if constexpr (TY == ORC_F16) {
+                    const uint32_t m0 = m >= 2 ? ~0u : m ? 0xFFFFu : 0u, m1 = m >= 4 ? ~0u : m == 3 ? 0xFFFFu : 0u;
+#pragma unroll
+                    for (int i = 0; i < DW; ++i) {
+                        v[i * 2 + s][q * 2] &= m0;
+                        v[i * 2 + s][q * 2 + 1] &= m1;
+                    }
+                } else
+                    vs[s * 2 + q] &= m >= 4 ? ~0u : (1u << (8 * m)) - 1u;
+            }
+    }
+    __device__ __forceinline__ void put(uint8_t* kt, uint8_t* vt, int wave, int lane) const {
+        kq_h2 sc = {};
+        if constexpr (TY != ORC_F16) sc = ka_scale_k(ks, wave);
+#pragma unroll
+        for (int i = 0; i < HD / 32; ++i) *(kq_h8*)(kt + (wave * (HD / 32) + i) * 1024 + lane * 16) = k.op(i, sc);
+#pragma unroll
+        for (int i = 0; i < DW; ++i)
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                kq_h8 o;
+                if constexpr (TY == ORC_F16) o = __builtin_bit_cast(kq_h8, v[i * 2 + s]);
+                else {
+                    const int sh = TY == ORC_KV_Q4 ? ((wave * DW + i) & 1) * 4 : 0;
+                    const u32x4& r = v[TY == ORC_KV_Q8 ? i : 0];
+                    uint32_t w0 = r[s * 2] >> sh, w1 = r[s * 2 + 1] >> sh;
+                    if constexpr (TY == ORC_KV_Q4) {
+                        w0 &= 0x0F0F0F0Fu;
+                        w1 &= 0x0F0F0F0Fu;
+                    }
+                    kq_h2 q[4];
+                    ka_cvt4(w0, ka_scale_v(vs[s * 2], 0), ka_scale_v(vs[s * 2], 2), (_Float16)ka_bias<TY>(), q[0], q[1]);
+                    ka_cvt4(w1, ka_scale_v(vs[s * 2 + 1], 0), ka_scale_v(vs[s * 2 + 1], 2), (_Float16)ka_bias<TY>(), q[2], q[3]);
+                    o = ka_join(q[0], q[1], q[2], q[3]);
+                }
+                *(kq_h8*)(vt + ((wave * DW + i) * 2 + s) * 1024 + lane * 16) = o;
+            }
+    }
+};
+
+template <int TY, int HD, int RT> __global__ __launch_bounds__(64 * kKaWaves, 2) void k_attn_kvq_tile(KaArgs a) {
+    constexpr int DT = HD / 16, KS = HD / 32, BB = kvq_block_bytes(TY, HD), M = 16 * RT * kKaWaves, TB = kKvBlock * HD * 2;
+    __shared__ __attribute__((aligned(16))) uint8_t sh[2][2][TB];
+    KaJob j;
+    if (!ka_job(a, M, j)) return;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 15, g = lane >> 4;
+    const bool direct = a.cp + a.co == 1;
+    if (j.b0 >= j.b1 && !direct) return;
+    const int nbp = (a.prefix + kKvBlock - 1) / kKvBlock;
+    const int w0 = j.r0 + wave * 16 * RT;  // the wave's first row
+
+    KaQ<TY, HD> q[RT];
+    KaRow st[RT];
+    int vis[RT];
+    kq_f4 o[RT][DT];
+#pragma unroll
+    for (int r = 0; r < RT; ++r) {
+        const int row = w0 + r * 16 + c, tok = row / a.group, hg = row - tok * a.group;
+        q[r].load(a.q + (int64_t)tok * a.ldq + (size_t)(j.kv * a.group + hg) * HD, row < j.r1, g);
+        vis[r] = j.seq < 0 ? 0 : min(j.start + tok - j.seq * a.n_tok + 1, j.len);
+#pragma unroll
+        for (int d = 0; d < DT; ++d) o[r][d] = kq_f4{0.f, 0.f, 0.f, 0.f};
+    }
+    // own rows that the wave's first and last row see
+    const int first_own = j.seq < 0 ? 0 : min(j.start + w0 / a.group - j.seq * a.n_tok + 1, j.len);
+    const int last_own = j.seq < 0 ? 0 : min(j.start + (min(w0 + 16 * RT, j.r1) - 1) / a.group - j.seq * a.n_tok + 1, j.len);
+    const bool rows = w0 < j.r1;
+    const uint8_t* pk = a.pk + (size_t)j.kv * (a.pctx / kKvBlock) * BB;
+    const uint8_t* pv = a.pv + (size_t)j.kv * (a.pctx / kKvBlock) * BB;
+    const size_t own = ((size_t)max(j.seq, 0) * a.n_kv + j.kv) * (a.ctx / kKvBlock) * BB;
+    KaStage<TY, HD> sg;
+    auto load = [&](int b) {
+        const bool pre = b < nbp;
+        sg.load(pre ? pk + (size_t)b * BB : a.kc + own + (size_t)(b - nbp) * BB,
+                pre ? pv + (size_t)b * BB : a.vc + own + (size_t)(b - nbp) * BB, wave, lane);
+    };
+    auto limit = [&](int b) { return b < nbp ? a.prefix - b * kKvBlock : j.len - (b - nbp) * kKvBlock; };
+    auto put = [&](int b, int buf) {
+        if (limit(b) < kKvBlock) sg.keep(limit(b), lane);
+        sg.put(sh[buf][0], sh[buf][1], wave, lane);
+    };
+    float sgn = 1.f;
+    if (j.b0 < j.b1) {
+        load(j.b0);
+        put(j.b0, 0);
+        load(min(j.b0 + 1, j.b1 - 1));
+    }
+    __syncthreads();
+    for (int b = j.b0; b < j.b1; ++b) {
+        const int cur = (b - j.b0) & 1;
+        const bool pre = b < nbp;
+        const int key0 = (pre ? b : b - nbp) * kKvBlock, lim = limit(b);
+        const uint8_t *kt = sh[cur][0] + lane * 16, *vt = sh[cur][1] + lane * 16;
+        if (rows && (pre || key0 < last_own)) {
+            kq_f4 s[RT][4];
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+#pragma unroll
+                for (int r = 0; r < RT; ++r) s[r][t] = kq_f4{0.f, 0.f, 0.f, 0.f};
+                kq_h8 k[KS];
+#pragma unroll
+                for (int i = 0; i < KS; ++i) k[i] = *(const kq_h8*)(kt + (t * KS + i) * 1024);
+#pragma unroll
+                for (int i = 0; i < KS; ++i)
+#pragma unroll
+                    for (int r = 0; r < RT; ++r) s[r][t] = ka_mfma(k[i], q[r].lo[i], s[r][t]);
+#pragma unroll
+                for (int i = 0; i < KS; ++i)
+#pragma unroll
+                    for (int r = 0; r < RT; ++r) s[r][t] = ka_mfma(k[i], q[r].hi[i], s[r][t]);
+            }
+            if (lim < kKvBlock || (!pre && first_own - key0 < kKvBlock)) {
+#pragma unroll
+                for (int r = 0; r < RT; ++r) {
+                    const int n = pre ? lim : min(lim, vis[r] - key0);
+#pragma unroll
+                    for (int t = 0; t < 4; ++t)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            if (t * 16 + g * 4 + i >= n) s[r][t][i] = -__builtin_inff();
+                }
+            }
+            sgn = -sgn;
+            const uint32_t sign = sgn < 0.f ? 0x80008000u : 0u;
+            u32x4 ph[RT][2], pl[RT][2];
+            float beta[RT];
+#pragma unroll
+            for (int r = 0; r < RT; ++r) beta[r] = -st[r].step(s[r], q[r].f, sign, ph[r], pl[r]);
+#pragma unroll
+            for (int d = 0; d < DT; ++d) {
+                const kq_h8 v0 = *(const kq_h8*)(vt + d * 2048), v1 = *(const kq_h8*)(vt + d * 2048 + 1024);
+                kq_f4 z[RT];
+#pragma unroll
+                for (int r = 0; r < RT; ++r) z[r] = ka_mfma(v0, __builtin_bit_cast(kq_h8, pl[r][0]), kq_f4{0.f, 0.f, 0.f, 0.f});
+#pragma unroll
+                for (int r = 0; r < RT; ++r) z[r] = ka_mfma(v1, __builtin_bit_cast(kq_h8, pl[r][1]), z[r]);
+#pragma unroll
+                for (int r = 0; r < RT; ++r) z[r] = ka_mfma(v0, __builtin_bit_cast(kq_h8, ph[r][0]), z[r]);
+#pragma unroll
+                for (int r = 0; r < RT; ++r) z[r] = ka_mfma(v1, __builtin_bit_cast(kq_h8, ph[r][1]), z[r]);
+#pragma unroll
+                for (int r = 0; r < RT; ++r)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) o[r][d][i] = __builtin_fmaf(o[r][d][i], beta[r], z[r][i]);
+            }
+        }
+        // the next block into the other buffer (read last before the barrier that ended the block before this one)
+        if (b + 1 < j.b1) {
+            put(b + 1, cur ^ 1);
+            load(min(b + 2, j.b1 - 1));
+        }
+        __syncthreads();
+    }
+#pragma unroll
+    for (int r = 0; r < RT; ++r) {
+        float l = st[r].l;
+        l += __shfl_xor(l, 16, 64);
+        l += __shfl_xor(l, 32, 64);
+        const int row = w0 + r * 16 + c;
+        if (row >= j.r1) continue;
+        const int tok = row / a.group, head = j.kv * a.group + (row - tok * a.group);
+        if (direct) {
+            const bool live = j.start >= 0 && j.start + (int64_t)(tok - j.seq * a.n_tok) < a.limit && l != 0.f;
+            const float inv = sgn * (TY == ORC_F16 ? 1.f : 0.0625f) / l;
+            float* out = a.out + (int64_t)tok * a.ldo + (size_t)head * HD + g * 4;
+#pragma unroll
+            for (int d = 0; d < DT; ++d) {
+                kq_f4 y = {0.f, 0.f, 0.f, 0.f};
+                if (live) y = o[r][d] * inv;
+                *(kq_f4*)(out + d * 16) = y;
+            }
+        } else {
+            const size_t at = (size_t)j.slot * a.n_rows + (size_t)tok * a.n_heads + head;
+#pragma unroll
+            for (int d = 0; d < DT; ++d) *(kq_f4*)(a.part_o + at * HD + d * 16 + g * 4) = o[r][d] * sgn;
+            if (g == 0) a.part_ml[at] = make_float2(st[r].m, l);
+        }
+    }
+}
+
 // ── the chunks' partial sums ─────────────────────────────────────────────────
-// One wave per row: out = sum over chunks of 2^(m_c - max) O_c over the same of l_c.
-template <int HD> __global__ __launch_bounds__(256) void k_attn_kvq_merge(KaArgs a, float unit) {
-    const int lane = threadIdx.x & 63;
-    const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (row >= a.n_rows) return;
-    constexpr int E = HD / 64;
-    const int tok = (int)(row / a.n_heads), head = (int)(row - (int64_t)tok * a.n_heads), seq = tok / a.n_tok;
-    const int start = kvq_start(a.d_pos, seq, a.pos_off, a.limit);
-    float* out = a.out + (int64_t)tok * a.ldo + (size_t)head * HD;
+// out = sum over chunks of 2^(m_c - max) O_c over the same of l_c, W waves a
+// row: the lanes form the chunks' weights side by side, then each wave adds
+// every W-th chunk.
+constexpr int kKaSlots = 1024;
+template <int HD, int W> __global__ __launch_bounds__(256) void k_attn_kvq_merge(KaArgs a, float unit) {
+    constexpr int R = 4 / W, E = HD / 64, N = W == 1 ? 16 : kKaSlots;  // rows of a workgroup
+    __shared__ float wt[R][N];
+    __shared__ float acc[W][HD];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, sub = wave / W;
+    const int64_t row = (int64_t)blockIdx.x * R + sub;
+    const bool some = row < a.n_rows;
+    const int tok = some ? (int)(row / a.n_heads) : 0, head = some ? (int)(row - (int64_t)tok * a.n_heads) : 0, seq = tok / a.n_tok;
+    const int start = kvq_start(a.d_pos, seq, a.pos_off, a.limit), n = a.cp + a.co;
+    const bool live = some && start >= 0 && start + (int64_t)(tok - seq * a.n_tok) < a.limit;
     float v[E] = {};
     float l = 0.f;
-    if (start >= 0 && start + (int64_t)(tok - seq * a.n_tok) < a.limit) {
+    if (live) {
         const int len = (int)min((int64_t)start + a.n_tok, (int64_t)a.limit);
         const int nbp = (a.prefix + kKvBlock - 1) / kKvBlock, first = a.shared ? nbp : 0;
         const int nb = nbp - first + (len + kKvBlock - 1) / kKvBlock;
         const int last = nbp - first + (start + tok - seq * a.n_tok) / kKvBlock;  // the row's last block
         float m = -__builtin_inff();
-        for (int pass = 0; pass < 2; ++pass)
-            for (int c = 0; c < a.cp + a.co; ++c) {
-                int b0, b1;
-                if (c < a.cp) ka_chunk(nbp, a.cp, c, b0, b1);
-                else ka_chunk(nb, a.co, c - a.cp, b0, b1);
-                if (b0 >= b1 || (c >= a.cp && b0 > last)) continue;
-                const size_t at = (size_t)c * a.n_rows + row;
-                const float2 ml = a.part_ml[at];
-                if (pass == 0) {
-                    m = fmaxf(m, ml.x);
-                    continue;
-                }
-                if (ml.y == 0.f) continue;
-                const float e = __builtin_amdgcn_exp2f(ml.x - m);
-                l += e * ml.y;
+        auto get = [&](int c) {  // (maximum, sum) of chunk c; (-inf, 0) where it holds nothing of the row
+            int b0, b1;
+            if (c < a.cp) ka_chunk(nbp, a.cp, c, b0, b1);
+            else ka_chunk(nb, a.co, c - a.cp, b0, b1);
+            if (c >= n || b0 >= b1 || (c >= a.cp && b0 > last)) return make_float2(-__builtin_inff(), 0.f);
+            return a.part_ml[(size_t)c * a.n_rows + row];
+        };
+        const float2 mine = get(lane);
+        m = mine.x;
+        for (int c = lane + 64; c < n; c += 64) m = fmaxf(m, get(c).x);
 #pragma unroll
-                for (int i = 0; i < E; ++i) v[i] += e * a.part_o[at * HD + lane + 64 * i];
-            }
+        for (int d = 32; d; d >>= 1) m = fmaxf(m, __shfl_xor(m, d, 64));
+        for (int c = lane; c < n; c += 64) {
+            const float2 ml = c == lane ? mine : get(c);
+            const float e = ml.y == 0.f ? 0.f : __builtin_amdgcn_exp2f(ml.x - m);
+            if (ml.y != 0.f) l += e * ml.y;
+            if (W == 1 || wave == 0) wt[sub][c] = e;
+        }
+#pragma unroll
+        for (int d = 32; d; d >>= 1) l += __shfl_xor(l, d, 64);
     }
+    __syncthreads();
+    if (live) {
+        const float* po = a.part_o + (size_t)row * HD + lane * E;
+#pragma unroll 4
+        for (int c = wave % W; c < n; c += W) {
+            const float e = wt[sub][c];
+            if (e == 0.f) continue;
+            const float* p = po + (size_t)c * a.n_rows * HD;
 #pragma unroll
-    for (int i = 0; i < E; ++i) out[lane + 64 * i] = l == 0.f ? 0.f : v[i] * (unit / l);
+            for (int i = 0; i < E; ++i) v[i] += e * p[i];
+        }
+    }
+    if constexpr (W > 1) {
+#pragma unroll
+        for (int i = 0; i < E; ++i) acc[wave][lane * E + i] = v[i];
+        __syncthreads();
+        if (wave) return;
+#pragma unroll
+        for (int w = 1; w < W; ++w)
+#pragma unroll
+            for (int i = 0; i < E; ++i) v[i] += acc[w][lane * E + i];
+    }
+    if (!some) return;
+    float* out = a.out + (int64_t)tok * a.ldo + (size_t)head * HD + lane * E;
+#pragma unroll
+    for (int i = 0; i < E; ++i) out[i] = l == 0.f ? 0.f : v[i] * (unit / l);
 }
 
 // ── host ─────────────────────────────────────────────────────────────────────
 struct KaPlan {
     bool shared;
-    int rt_p, rt_o, tiles_p, cp, tiles_o, co;
+    int m_p, m_o;  // rows of a workgroup: 16 or 32 (the waves share out the keys), 64 or 128 (they share the operands)
+    int tiles_p, cp, tiles_o, co;
     size_t rows;
     int slots() const { return cp + co; }
     size_t bytes(int hd) const { return slots() > 1 ? (size_t)slots() * rows * (4 * (size_t)hd + 8) : 0; }
@@ -487,10 +733,12 @@ struct KaPlan {
 
 static int ka_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 
+static int ka_rows(int64_t rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128; }
+
 // Chunks of nb key blocks for `base` workgroups' worth of row tiles: about two
-// workgroups per CU, and a block for every wave.
+// workgroups per CU, at least four blocks each (one for every wave).
 static int ka_chunks(int64_t base, int nb) {
-    return (int)std::max<int64_t>(1, std::min<int64_t>((512 + base - 1) / base, nb / kKaWaves));
+    return (int)std::max<int64_t>(1, std::min<int64_t>(512 / base, nb / kKaWaves));
 }
 
 static KaPlan ka_plan(int n_seq, int n_tok, int n_heads, int n_kv, int prefix_len, int pos_limit) {
@@ -498,22 +746,36 @@ static KaPlan ka_plan(int n_seq, int n_tok, int n_heads, int n_kv, int prefix_le
     const int64_t group = n_heads / n_kv, rows_o = n_tok * group, rows_p = n_seq * rows_o;
     p.rows = (size_t)n_seq * n_tok * n_heads;
     const int nbp = ka_div(prefix_len, kKvBlock), nbo = ka_div(pos_limit, kKvBlock);
-    p.shared = prefix_len > 0 && n_seq > 1;
-    p.rt_o = p.rt_p = (p.shared ? rows_p : rows_o) > 16 ? 2 : 1;
-    p.tiles_o = ka_div(rows_o, 16 * p.rt_o);
+    // with this many rows each, sequences gain nothing from common tiles
+    p.shared = prefix_len > 0 && n_seq > 1 && rows_o < 128;
+    p.m_o = ka_rows(rows_o);
+    p.tiles_o = ka_div(rows_o, p.m_o);
     p.co = ka_chunks((int64_t)n_seq * n_kv * p.tiles_o, p.shared ? nbo : nbp + nbo);
     if (p.shared) {
-        p.tiles_p = ka_div(rows_p, 16 * p.rt_p);
+        p.m_p = ka_rows(rows_p);
+        p.tiles_p = ka_div(rows_p, p.m_p);
         p.cp = ka_chunks((int64_t)n_kv * p.tiles_p, nbp);
     }
     return p;
 }
 
+template <int TY, int HD> static void ka_jobs(int m, int64_t job0, int64_t jobs, KaArgs a, hipStream_t s) {
+    a.job0 = (int)job0;
+    a.jobs = (int)jobs;
+    const dim3 grid((unsigned)((jobs + 7) / 8 * 8)), wg(64 * kKaWaves);
+    if (m == 16) hipLaunchKernelGGL((k_attn_kvq<TY, HD, 1>), grid, wg, 0, s, a);
+    else if (m == 32) hipLaunchKernelGGL((k_attn_kvq<TY, HD, 2>), grid, wg, 0, s, a);
+    else if (m == 64) hipLaunchKernelGGL((k_attn_kvq_tile<TY, HD, 1>), grid, wg, 0, s, a);
+    else hipLaunchKernelGGL((k_attn_kvq_tile<TY, HD, 2>), grid, wg, 0, s, a);
+}
+
 template <int TY, int HD> static void ka_launch(const KaPlan& p, const KaArgs& a, hipStream_t s) {
-    const int64_t jobs = (int64_t)a.n_kv * p.cp * p.tiles_p + (int64_t)a.n_seq * a.n_kv * p.co * p.tiles_o;
-    const dim3 grid((unsigned)((jobs + 7) / 8 * 8));
-    if (p.rt_o == 1) hipLaunchKernelGGL((k_attn_kvq<TY, HD, 1>), grid, dim3(64 * kKaWaves), 0, s, a);
-    else hipLaunchKernelGGL((k_attn_kvq<TY, HD, 2>), grid, dim3(64 * kKaWaves), 0, s, a);
+    const int64_t jobs_p = (int64_t)a.n_kv * p.cp * p.tiles_p, jobs_o = (int64_t)a.n_seq * a.n_kv * p.co * p.tiles_o;
+    if (p.shared && p.m_p != p.m_o) {
+        ka_jobs<TY, HD>(p.m_p, 0, jobs_p, a, s);
+        ka_jobs<TY, HD>(p.m_o, jobs_p, jobs_o, a, s);
+    } else
+        ka_jobs<TY, HD>(p.m_o, 0, jobs_p + jobs_o, a, s);
 }
 
 }  // namespace orc
@@ -557,7 +819,7 @@ extern "C" int orc_attn_kvq(int type, const float* d_q, int ldq, int n_seq, int 
     if (jobs > 0xffffff00ll / 256 - 8) return set_error(ORC_E_INVALID, "attn_kvq: too many rows");
     KaArgs a{d_q, ldq, n_seq, n_tok, n_heads, n_kv, n_heads / n_kv, (const uint8_t*)d_pk, (const uint8_t*)d_pv,
              (const uint8_t*)d_kc, (const uint8_t*)d_vc, prefix_len, prefix_ctx, ctx, d_pos, pos_off, pos_limit, d_out,
-             ldo, nullptr, nullptr, (int)p.rows, p.shared, p.tiles_p, p.cp, p.tiles_o, p.co};
+             ldo, nullptr, nullptr, (int)p.rows, p.shared, p.tiles_p, p.cp, p.tiles_o, p.co, 0, 0};
     if (bytes) {
         a.part_o = (float*)d_work;
         a.part_ml = (float2*)((uint8_t*)d_work + (size_t)p.slots() * p.rows * head_dim * 4);
@@ -572,10 +834,12 @@ extern "C" int orc_attn_kvq(int type, const float* d_q, int ldq, int n_seq, int 
     else go(std::integral_constant<int, ORC_KV_Q4>());
     ORC_LAUNCH_CHECK();
     if (p.slots() > 1) {
-        const dim3 grid((unsigned)ka_div((int64_t)p.rows, 4));
         const float unit = type == ORC_F16 ? 1.f : 0.0625f;
-        if (head_dim == 64) hipLaunchKernelGGL(k_attn_kvq_merge<64>, grid, dim3(256), 0, st, a, unit);
-        else hipLaunchKernelGGL(k_attn_kvq_merge<128>, grid, dim3(256), 0, st, a, unit);
+        auto merge = [&](auto kernel, int rows) {
+            hipLaunchKernelGGL(kernel, dim3((unsigned)ka_div((int64_t)p.rows, rows)), dim3(256), 0, st, a, unit);
+        };
+        if (p.slots() <= 16) head_dim == 64 ? merge(k_attn_kvq_merge<64, 1>, 4) : merge(k_attn_kvq_merge<128, 1>, 4);
+        else head_dim == 64 ? merge(k_attn_kvq_merge<64, 4>, 1) : merge(k_attn_kvq_merge<128, 4>, 1);
         ORC_LAUNCH_CHECK();
     }
     return ORC_OK;
