@@ -34,9 +34,9 @@ struct KaArgs {
     float* part_o;   // [slot][row][hd], row = token n_heads + head
     float2* part_ml; // [slot][row] (maximum, sum)
     int n_rows;      // n_seq n_tok n_heads
-    // jobs: prefix ones (shared form only), then own ones; a launch takes `jobs` of them from `job0` on
+    // jobs: prefix ones (shared form only), then own ones
     int shared, tiles_p, cp, tiles_o, co;
-    int job0, jobs;
+    int jobs_p, jobs_o;
 };
 
 // Blocks [b0, b1) of chunk c of n chunks over nb blocks.
@@ -53,31 +53,31 @@ struct KaJob {
     int kv, seq, r0, r1, b0, b1, slot, start, len;
 };
 
-__device__ __forceinline__ bool ka_job(const KaArgs& a, int m_rows, KaJob& j) {
-    // work items in order on each XCD: the row tiles of one chunk, which read the same keys, share its L2
-    const int jobs_p = a.shared ? a.n_kv * a.cp * a.tiles_p : 0, per = (a.jobs + 7) / 8;
-    int w = (int)(blockIdx.x & 7) * per + (int)(blockIdx.x >> 3);
-    if (w >= a.jobs) return false;
-    w += a.job0;
+__device__ __forceinline__ bool ka_job(const KaArgs& a, int m_p, int m_o, KaJob& j) {
+    // Every XCD takes an eighth of the prefix jobs, then an eighth of the own ones, each in order: the row tiles of one
+    // chunk, which read the same keys, share its L2.
+    const int per_p = (a.jobs_p + 7) / 8, per_o = (a.jobs_o + 7) / 8, x = blockIdx.x & 7, i = blockIdx.x >> 3;
+    const bool pre = i < per_p;
+    int w = pre ? x * per_p + i : x * per_o + i - per_p;
+    if (w >= (pre ? a.jobs_p : a.jobs_o)) return false;
     const int nbp = (a.prefix + kKvBlock - 1) / kKvBlock;
-    if (w < jobs_p) {
+    if (pre) {
         const int tile = w % a.tiles_p, c = w / a.tiles_p % a.cp;
         j.kv = w / a.tiles_p / a.cp;
         j.seq = -1;
-        j.r0 = tile * m_rows;
-        j.r1 = min(j.r0 + m_rows, a.n_seq * a.n_tok * a.group);
+        j.r0 = tile * m_p;
+        j.r1 = min(j.r0 + m_p, a.n_seq * a.n_tok * a.group);
         j.start = j.len = 0;
         j.slot = c;
         ka_chunk(nbp, a.cp, c, j.b0, j.b1);
         return true;
     }
-    w -= jobs_p;
     const int tile = a.tiles_o - 1 - w % a.tiles_o, c = w / a.tiles_o % a.co;  // the longest rows first
     const int sk = w / a.tiles_o / a.co, rows = a.n_tok * a.group;
     j.seq = sk / a.n_kv;
     j.kv = sk % a.n_kv;
-    j.r0 = j.seq * rows + tile * m_rows;
-    j.r1 = min(j.r0 + m_rows, (j.seq + 1) * rows);
+    j.r0 = j.seq * rows + tile * m_o;
+    j.r1 = min(j.r0 + m_o, (j.seq + 1) * rows);
     j.start = kvq_start(a.d_pos, j.seq, a.pos_off, a.limit);
     j.len = j.start < 0 ? 0 : (int)min((int64_t)j.start + a.n_tok, (int64_t)a.limit);
     j.slot = a.cp + c;
@@ -147,9 +147,9 @@ template <int TY, int HD> struct KaK {
 __device__ __forceinline__ kq_h2 ka_scale_k(uint32_t w, int T) {
     return __builtin_bit_cast(kq_h2, __builtin_amdgcn_perm(0u, w, 0x000C000Cu | (T << 8) | (T << 24)) >> 1);
 }
-// Scales of bytes e, e + 1 of w.
-__device__ __forceinline__ kq_h2 ka_scale_v(uint32_t w, int e) {
-    return __builtin_bit_cast(kq_h2, __builtin_amdgcn_perm(0u, w, 0x000C000Cu | (e << 8) | ((e + 1) << 24)) >> 1);
+// Scales of bytes e, e + 1 of w; sign 0x80008000 negates them.
+__device__ __forceinline__ kq_h2 ka_scale_v(uint32_t w, int e, uint32_t sign = 0) {
+    return __builtin_bit_cast(kq_h2, __builtin_amdgcn_perm(0u, w, 0x000C000Cu | (e << 8) | ((e + 1) << 24)) >> 1 ^ sign);
 }
 
 // V bytes of one dim tile (both tiles of a pair for 4 bits) of a lane.
@@ -209,11 +209,21 @@ template <int TY, int HD> struct KaV {
     }
 };
 
-// Two fp16 halves of a and b.
-__device__ __forceinline__ uint32_t ka_split(float a, float b, uint32_t& lo) {
+// Larger of two by v_maximum3_f32: takes the matrix cores' results as they come, which v_max_f32 does not (a move each
+// to quiet what might be a signalling NaN), and hands a NaN on.
+__device__ __forceinline__ float ka_max(float a, float b) { return __builtin_elementwise_maximum(a, b); }
+
+// Two fp16 halves of a and b. `minus` is -1 where the compiler does not see it, so that the rest is one v_fma_mix_f32
+// (which widens its fp16 factor) instead of a conversion and a subtraction.
+__device__ __forceinline__ uint32_t ka_split(float a, float b, float minus, uint32_t& lo) {
     const kq_h2 hi = __builtin_bit_cast(kq_h2, __builtin_amdgcn_cvt_pkrtz(a, b));
-    lo = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(a - (float)hi.x, b - (float)hi.y));
+    lo = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(__builtin_fmaf((float)hi.x, minus, a), __builtin_fmaf((float)hi.y, minus, b)));
     return __builtin_bit_cast(uint32_t, hi);
+}
+__device__ __forceinline__ float ka_minus() {
+    float m = -1.f;
+    asm("" : "+s"(m));
+    return m;
 }
 
 // A query row as operands: its head dims (hd / 4 per lane group) times a power
@@ -245,7 +255,7 @@ template <int TY, int HD> struct KaQ {
             uint32_t h[4], l[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-                h[e] = ka_split(ldexpf(v[j * 8 + 2 * e], ex), ldexpf(v[j * 8 + 2 * e + 1], ex), l[e]);
+                h[e] = ka_split(ldexpf(v[j * 8 + 2 * e], ex), ldexpf(v[j * 8 + 2 * e + 1], ex), -1.f, l[e]);
             hi[j] = __builtin_bit_cast(kq_h8, u32x4{h[0], h[1], h[2], h[3]});
             lo[j] = __builtin_bit_cast(kq_h8, u32x4{l[0], l[1], l[2], l[3]});
         }
@@ -260,14 +270,21 @@ __device__ __forceinline__ kq_f4 ka_mfma(kq_h8 a, kq_h8 b, kq_f4 c) {
 // each sums its own keys).
 struct KaRow {
     float m = -__builtin_inff(), l = 0.f;
-    // scores s of the lane's 16 keys -> weights times 2^15 and sign; returns what the sums so far are scaled by
-    __device__ __forceinline__ float step(kq_f4 (&s)[4], float f, uint32_t sign, u32x4 (&hi)[2], u32x4 (&lo)[2]) {
-        float mx = fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3]));
-#pragma unroll
-        for (int t = 1; t < 4; ++t) mx = fmaxf(fmaxf(mx, fmaxf(s[t][0], s[t][1])), fmaxf(s[t][2], s[t][3]));
-        mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
-        mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-        const float mn = fmaxf(m, mx * f), ref = mn == -__builtin_inff() ? 0.f : mn;
+    // scores s of the lane's 16 keys -> weights times 2^15 (SIGN: and the sign bit); returns what the sums so far are
+    // scaled by
+    template <bool SIGN>
+    __device__ __forceinline__ float step(kq_f4 (&s)[4], float f, float minus, uint32_t sign, u32x4 (&hi)[2], u32x4 (&lo)[2]) {
+        float mx = ka_max(ka_max(s[0][0], s[0][1]), s[0][2]);
+        mx = ka_max(ka_max(mx, s[0][3]), s[1][0]);
+        mx = ka_max(ka_max(mx, s[1][1]), s[1][2]);
+        mx = ka_max(ka_max(mx, s[1][3]), s[2][0]);
+        mx = ka_max(ka_max(mx, s[2][1]), s[2][2]);
+        mx = ka_max(ka_max(mx, s[2][3]), s[3][0]);
+        mx = ka_max(ka_max(mx, s[3][1]), s[3][2]);
+        mx = ka_max(mx, s[3][3]);
+        mx = ka_max(ka_max(mx, __shfl_xor(mx, 16, 64)), __shfl_xor(mx, 32, 64));
+        mx = ka_max(mx, __shfl_xor(mx, 48, 64));
+        const float mn = ka_max(m, mx * f), ref = mn == -__builtin_inff() ? 0.f : mn;
         const float alpha = __builtin_amdgcn_exp2f(m - ref);
         m = mn;
         float sum = 0.f;
@@ -279,12 +296,12 @@ struct KaRow {
                 p[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][i], f, 15.f - ref));
                 sum += p[i];
             }
-            uint32_t l0, l1;
-            const uint32_t h0 = ka_split(p[0], p[1], l0), h1 = ka_split(p[2], p[3], l1);
-            hi[t / 2][(t & 1) * 2] = h0 ^ sign;
-            hi[t / 2][(t & 1) * 2 + 1] = h1 ^ sign;
-            lo[t / 2][(t & 1) * 2] = l0 ^ sign;
-            lo[t / 2][(t & 1) * 2 + 1] = l1 ^ sign;
+            uint32_t l0, l1, h0 = ka_split(p[0], p[1], minus, l0), h1 = ka_split(p[2], p[3], minus, l1);
+            if (SIGN) h0 ^= sign, h1 ^= sign, l0 ^= sign, l1 ^= sign;
+            hi[t / 2][(t & 1) * 2] = h0;
+            hi[t / 2][(t & 1) * 2 + 1] = h1;
+            lo[t / 2][(t & 1) * 2] = l0;
+            lo[t / 2][(t & 1) * 2 + 1] = l1;
         }
         l = l * alpha + sum;
         return alpha;
@@ -294,12 +311,14 @@ struct KaRow {
 // ── few rows: the waves share out the keys ───────────────────────────────────
 // A workgroup takes 16 RT rows; its waves take every fourth key block each,
 // straight from memory to operands, and join their sums at the end.
-template <int TY, int HD, int RT> __global__ __launch_bounds__(64 * kKaWaves) void k_attn_kvq(KaArgs a) {
+template <int HD, int RT> struct KaStreamLds {
+    float o[kKaWaves][16 * RT][HD + 4];
+    float2 ml[kKaWaves][16 * RT];
+};
+
+template <int TY, int HD, int RT>
+__device__ __forceinline__ void ka_stream(const KaArgs& a, const KaJob& j, KaStreamLds<HD, RT>& sh) {
     constexpr int DT = HD / 16, KS = HD / 32, BB = kvq_block_bytes(TY, HD), M = 16 * RT;
-    __shared__ float sh_o[kKaWaves][M][HD + 4];
-    __shared__ float2 sh_ml[kKaWaves][M];
-    KaJob j;
-    if (!ka_job(a, M, j)) return;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = lane & 15, g = lane >> 4;
     const bool direct = a.cp + a.co == 1;
     if (j.b0 >= j.b1 && !direct) return;
@@ -321,6 +340,7 @@ template <int TY, int HD, int RT> __global__ __launch_bounds__(64 * kKaWaves) vo
     const uint8_t* pk = a.pk + (size_t)j.kv * (a.pctx / kKvBlock) * BB;
     const uint8_t* pv = a.pv + (size_t)j.kv * (a.pctx / kKvBlock) * BB;
     const size_t own = ((size_t)max(j.seq, 0) * a.n_kv + j.kv) * (a.ctx / kKvBlock) * BB;
+    const float minus = ka_minus();
     float sgn = 1.f;
     for (int b = j.b0 + wave; b < j.b1; b += kKaWaves) {
         const bool pre = b < nbp;
@@ -369,7 +389,7 @@ template <int TY, int HD, int RT> __global__ __launch_bounds__(64 * kKaWaves) vo
         u32x4 ph[RT][2], pl[RT][2];
         float beta[RT];
 #pragma unroll
-        for (int r = 0; r < RT; ++r) beta[r] = -st[r].step(s[r], q[r].f, sign, ph[r], pl[r]);
+        for (int r = 0; r < RT; ++r) beta[r] = -st[r].template step<true>(s[r], q[r].f, minus, sign, ph[r], pl[r]);
 #pragma unroll
         for (int d = 0; d < DT; ++d) {
             const kq_h8 v0 = vr.op(d, 0), v1 = vr.op(d, 1);
@@ -392,34 +412,34 @@ template <int TY, int HD, int RT> __global__ __launch_bounds__(64 * kKaWaves) vo
         l += __shfl_xor(l, 16, 64);
         l += __shfl_xor(l, 32, 64);
         st[r].l = l;
-        if (g == 0) sh_ml[wave][r * 16 + c] = make_float2(st[r].m, l);
+        if (g == 0) sh.ml[wave][r * 16 + c] = make_float2(st[r].m, l);
     }
     __syncthreads();
 #pragma unroll
     for (int r = 0; r < RT; ++r) {
-        float mm = sh_ml[0][r * 16 + c].x;
+        float mm = sh.ml[0][r * 16 + c].x;
 #pragma unroll
-        for (int w = 1; w < kKaWaves; ++w) mm = fmaxf(mm, sh_ml[w][r * 16 + c].x);
+        for (int w = 1; w < kKaWaves; ++w) mm = fmaxf(mm, sh.ml[w][r * 16 + c].x);
         const float e = st[r].l == 0.f ? 0.f : __builtin_amdgcn_exp2f(st[r].m - mm) * sgn;
 #pragma unroll
         for (int d = 0; d < DT; ++d)
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-                sh_o[wave][r * 16 + c][d * 16 + g * 4 + i] = st[r].l == 0.f ? 0.f : o[r][d][i] * e;
+                sh.o[wave][r * 16 + c][d * 16 + g * 4 + i] = st[r].l == 0.f ? 0.f : o[r][d][i] * e;
     }
     __syncthreads();
     for (int it = tid; it < M * (HD / 4); it += 64 * kKaWaves) {
         const int rr = it / (HD / 4), d = it % (HD / 4) * 4, row = j.r0 + rr;
         if (row >= j.r1) continue;
-        float mm = sh_ml[0][rr].x, l = 0.f;
+        float mm = sh.ml[0][rr].x, l = 0.f;
 #pragma unroll
-        for (int w = 1; w < kKaWaves; ++w) mm = fmaxf(mm, sh_ml[w][rr].x);
+        for (int w = 1; w < kKaWaves; ++w) mm = fmaxf(mm, sh.ml[w][rr].x);
         kq_f4 v = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int w = 0; w < kKaWaves; ++w) {
-            const float2 ml = sh_ml[w][rr];
+            const float2 ml = sh.ml[w][rr];
             if (ml.y != 0.f) l += ml.y * __builtin_amdgcn_exp2f(ml.x - mm);
-            v += *(const kq_f4*)&sh_o[w][rr][d];
+            v += *(const kq_f4*)&sh.o[w][rr][d];
         }
         const int tok = row / a.group, head = j.kv * a.group + (row - tok * a.group);
         if (direct) {
@@ -480,7 +500,8 @@ template <int TY, int HD> struct KaStage {
                     vs[s * 2 + q] &= m >= 4 ? ~0u : (1u << (8 * m)) - 1u;
             }
     }
-    __device__ __forceinline__ void put(uint8_t* kt, uint8_t* vt, int wave, int lane) const {
+    // sign: 0x80008000 negates the block's V
+    __device__ __forceinline__ void put(uint8_t* kt, uint8_t* vt, int wave, int lane, uint32_t sign) const {
         kq_h2 sc = {};
         if constexpr (TY != ORC_F16) sc = ka_scale_k(ks, wave);
 #pragma unroll
@@ -490,7 +511,7 @@ template <int TY, int HD> struct KaStage {
 #pragma unroll
             for (int s = 0; s < 2; ++s) {
                 kq_h8 o;
-                if constexpr (TY == ORC_F16) o = __builtin_bit_cast(kq_h8, v[i * 2 + s]);
+                if constexpr (TY == ORC_F16) o = __builtin_bit_cast(kq_h8, v[i * 2 + s] ^ sign);
                 else {
                     const int sh = TY == ORC_KV_Q4 ? ((wave * DW + i) & 1) * 4 : 0;
                     const u32x4& r = v[TY == ORC_KV_Q8 ? i : 0];
@@ -500,8 +521,8 @@ template <int TY, int HD> struct KaStage {
                         w1 &= 0x0F0F0F0Fu;
                     }
                     kq_h2 q[4];
-                    ka_cvt4(w0, ka_scale_v(vs[s * 2], 0), ka_scale_v(vs[s * 2], 2), (_Float16)ka_bias<TY>(), q[0], q[1]);
-                    ka_cvt4(w1, ka_scale_v(vs[s * 2 + 1], 0), ka_scale_v(vs[s * 2 + 1], 2), (_Float16)ka_bias<TY>(), q[2], q[3]);
+                    ka_cvt4(w0, ka_scale_v(vs[s * 2], 0, sign), ka_scale_v(vs[s * 2], 2, sign), (_Float16)ka_bias<TY>(), q[0], q[1]);
+                    ka_cvt4(w1, ka_scale_v(vs[s * 2 + 1], 0, sign), ka_scale_v(vs[s * 2 + 1], 2, sign), (_Float16)ka_bias<TY>(), q[2], q[3]);
                     o = ka_join(q[0], q[1], q[2], q[3]);
                 }
                 *(kq_h8*)(vt + ((wave * DW + i) * 2 + s) * 1024 + lane * 16) = o;
@@ -509,11 +530,13 @@ template <int TY, int HD> struct KaStage {
     }
 };
 
-template <int TY, int HD, int RT> __global__ __launch_bounds__(64 * kKaWaves, 2) void k_attn_kvq_tile(KaArgs a) {
-    constexpr int DT = HD / 16, KS = HD / 32, BB = kvq_block_bytes(TY, HD), M = 16 * RT * kKaWaves, TB = kKvBlock * HD * 2;
-    __shared__ __attribute__((aligned(16))) uint8_t sh[2][2][TB];
-    KaJob j;
-    if (!ka_job(a, M, j)) return;
+template <int HD> struct KaTileLds {
+    uint8_t t[2][2][kKvBlock * HD * 2];  // [buffer][K, V]
+};
+
+template <int TY, int HD, int RT>
+__device__ __forceinline__ void ka_tile(const KaArgs& a, const KaJob& j, KaTileLds<HD>& sh) {
+    constexpr int DT = HD / 16, KS = HD / 32, BB = kvq_block_bytes(TY, HD);
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 15, g = lane >> 4;
     const bool direct = a.cp + a.co == 1;
     if (j.b0 >= j.b1 && !direct) return;
@@ -548,8 +571,9 @@ template <int TY, int HD, int RT> __global__ __launch_bounds__(64 * kKaWaves, 2)
     auto limit = [&](int b) { return b < nbp ? a.prefix - b * kKvBlock : j.len - (b - nbp) * kKvBlock; };
     auto put = [&](int b, int buf) {
         if (limit(b) < kKvBlock) sg.keep(limit(b), lane);
-        sg.put(sh[buf][0], sh[buf][1], wave, lane);
+        sg.put(sh.t[buf][0], sh.t[buf][1], wave, lane, buf ? 0u : 0x80008000u);
     };
+    const float minus = ka_minus();
     float sgn = 1.f;
     if (j.b0 < j.b1) {
         load(j.b0);
@@ -561,8 +585,9 @@ template <int TY, int HD, int RT> __global__ __launch_bounds__(64 * kKaWaves, 2)
         const int cur = (b - j.b0) & 1;
         const bool pre = b < nbp;
         const int key0 = (pre ? b : b - nbp) * kKvBlock, lim = limit(b);
-        const uint8_t *kt = sh[cur][0] + lane * 16, *vt = sh[cur][1] + lane * 16;
+        const uint8_t *kt = sh.t[cur][0] + lane * 16, *vt = sh.t[cur][1] + lane * 16;
         if (rows && (pre || key0 < last_own)) {
+            sgn = cur ? 1.f : -1.f;
             kq_f4 s[RT][4];
 #pragma unroll
             for (int t = 0; t < 4; ++t) {
@@ -591,12 +616,10 @@ template <int TY, int HD, int RT> __global__ __launch_bounds__(64 * kKaWaves, 2)
                             if (t * 16 + g * 4 + i >= n) s[r][t][i] = -__builtin_inff();
                 }
             }
-            sgn = -sgn;
-            const uint32_t sign = sgn < 0.f ? 0x80008000u : 0u;
             u32x4 ph[RT][2], pl[RT][2];
             float beta[RT];
 #pragma unroll
-            for (int r = 0; r < RT; ++r) beta[r] = -st[r].step(s[r], q[r].f, sign, ph[r], pl[r]);
+            for (int r = 0; r < RT; ++r) beta[r] = -st[r].template step<false>(s[r], q[r].f, minus, 0u, ph[r], pl[r]);
 #pragma unroll
             for (int d = 0; d < DT; ++d) {
                 const kq_h8 v0 = *(const kq_h8*)(vt + d * 2048), v1 = *(const kq_h8*)(vt + d * 2048 + 1024);
@@ -647,6 +670,31 @@ template <int TY, int HD, int RT> __global__ __launch_bounds__(64 * kKaWaves, 2)
             if (g == 0) a.part_ml[at] = make_float2(st[r].m, l);
         }
     }
+}
+
+// ── kernels ──────────────────────────────────────────────────────────────────
+template <int TY, int HD, int RT> __global__ __launch_bounds__(64 * kKaWaves) void k_attn_kvq(KaArgs a) {
+    __shared__ __attribute__((aligned(16))) KaStreamLds<HD, RT> sh;
+    KaJob j;
+    if (ka_job(a, 16 * RT, 16 * RT, j)) ka_stream<TY, HD, RT>(a, j, sh);
+}
+
+template <int TY, int HD, int RT> __global__ __launch_bounds__(64 * kKaWaves, 2) void k_attn_kvq_tile(KaArgs a) {
+    __shared__ __attribute__((aligned(16))) KaTileLds<HD> sh;
+    KaJob j;
+    if (ka_job(a, 64 * RT, 64 * RT, j)) ka_tile<TY, HD, RT>(a, j, sh);
+}
+
+// Prefix jobs of many rows and own jobs of few in one launch: the own ones fill the CUs that the prefix leaves idle.
+template <int TY, int HD, int RP, int RO> __global__ __launch_bounds__(64 * kKaWaves, 2) void k_attn_kvq_both(KaArgs a) {
+    __shared__ __attribute__((aligned(16))) union {
+        KaTileLds<HD> t;
+        KaStreamLds<HD, RO> s;
+    } sh;
+    KaJob j;
+    if (!ka_job(a, 64 * RP, 16 * RO, j)) return;
+    if (j.seq < 0) ka_tile<TY, HD, RP>(a, j, sh.t);
+    else ka_stream<TY, HD, RO>(a, j, sh.s);
 }
 
 // ── the chunks' partial sums ─────────────────────────────────────────────────
@@ -733,12 +781,10 @@ struct KaPlan {
 
 static int ka_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 
-static int ka_rows(int64_t rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128; }
-
-// Chunks of nb key blocks for `base` workgroups' worth of row tiles: about two
-// workgroups per CU, at least four blocks each (one for every wave).
-static int ka_chunks(int64_t base, int nb) {
-    return (int)std::max<int64_t>(1, std::min<int64_t>(512 / base, nb / kKaWaves));
+// Chunks of nb key blocks for `base` workgroups' worth of row tiles: about two workgroups per CU, at least `least`
+// blocks each.
+static int ka_chunks(int64_t base, int nb, int least) {
+    return (int)std::max<int64_t>(1, std::min<int64_t>(512 / base, nb / least));
 }
 
 static KaPlan ka_plan(int n_seq, int n_tok, int n_heads, int n_kv, int prefix_len, int pos_limit) {
@@ -746,36 +792,31 @@ static KaPlan ka_plan(int n_seq, int n_tok, int n_heads, int n_kv, int prefix_le
     const int64_t group = n_heads / n_kv, rows_o = n_tok * group, rows_p = n_seq * rows_o;
     p.rows = (size_t)n_seq * n_tok * n_heads;
     const int nbp = ka_div(prefix_len, kKvBlock), nbo = ka_div(pos_limit, kKvBlock);
+    static int e_min = getenv("KA_MIN") ? atoi(getenv("KA_MIN")) : 2, e_mins = getenv("KA_MINS") ? atoi(getenv("KA_MINS")) : 4;
     // with this many rows each, sequences gain nothing from common tiles
     p.shared = prefix_len > 0 && n_seq > 1 && rows_o < 128;
-    p.m_o = ka_rows(rows_o);
-    p.tiles_o = ka_div(rows_o, p.m_o);
-    p.co = ka_chunks((int64_t)n_seq * n_kv * p.tiles_o, p.shared ? nbo : nbp + nbo);
     if (p.shared) {
-        p.m_p = ka_rows(rows_p);
+        p.m_p = rows_p <= 16 ? 16 : rows_p <= 32 ? 32 : n_kv * (int64_t)ka_div(rows_p, 128) * (nbp / 8) >= 512 ? 128 : 64;
+        p.m_o = p.m_p <= 32 ? p.m_p : rows_o <= 16 ? 16 : rows_o <= 32 ? 32 : p.m_p;
         p.tiles_p = ka_div(rows_p, p.m_p);
-        p.cp = ka_chunks((int64_t)n_kv * p.tiles_p, nbp);
-    }
+        p.cp = ka_chunks((int64_t)n_kv * p.tiles_p, nbp, p.m_p <= 32 ? e_mins : e_min);
+    } else
+        p.m_o = rows_o <= 16 ? 16 : rows_o <= 32 ? 32 : (int64_t)n_seq * n_kv * ka_div(rows_o, 128) >= 1024 ? 128 : 64;
+    if (getenv("KA_MO")) p.m_o = atoi(getenv("KA_MO"));
+    p.tiles_o = ka_div(rows_o, p.m_o);
+    p.co = ka_chunks((int64_t)n_seq * n_kv * p.tiles_o, p.shared ? nbo : nbp + nbo, p.m_o <= 32 ? e_mins : e_min);
     return p;
 }
 
-template <int TY, int HD> static void ka_jobs(int m, int64_t job0, int64_t jobs, KaArgs a, hipStream_t s) {
-    a.job0 = (int)job0;
-    a.jobs = (int)jobs;
-    const dim3 grid((unsigned)((jobs + 7) / 8 * 8)), wg(64 * kKaWaves);
-    if (m == 16) hipLaunchKernelGGL((k_attn_kvq<TY, HD, 1>), grid, wg, 0, s, a);
-    else if (m == 32) hipLaunchKernelGGL((k_attn_kvq<TY, HD, 2>), grid, wg, 0, s, a);
-    else if (m == 64) hipLaunchKernelGGL((k_attn_kvq_tile<TY, HD, 1>), grid, wg, 0, s, a);
-    else hipLaunchKernelGGL((k_attn_kvq_tile<TY, HD, 2>), grid, wg, 0, s, a);
-}
-
 template <int TY, int HD> static void ka_launch(const KaPlan& p, const KaArgs& a, hipStream_t s) {
-    const int64_t jobs_p = (int64_t)a.n_kv * p.cp * p.tiles_p, jobs_o = (int64_t)a.n_seq * a.n_kv * p.co * p.tiles_o;
-    if (p.shared && p.m_p != p.m_o) {
-        ka_jobs<TY, HD>(p.m_p, 0, jobs_p, a, s);
-        ka_jobs<TY, HD>(p.m_o, jobs_p, jobs_o, a, s);
-    } else
-        ka_jobs<TY, HD>(p.m_o, 0, jobs_p + jobs_o, a, s);
+    auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(8 * ((unsigned)(a.jobs_p + 7) / 8 + (unsigned)(a.jobs_o + 7) / 8)), dim3(64 * kKaWaves), 0, s, a); };
+    if (!p.shared || p.m_p == p.m_o) {
+        if (p.m_o == 16) go(k_attn_kvq<TY, HD, 1>);
+        else if (p.m_o == 32) go(k_attn_kvq<TY, HD, 2>);
+        else if (p.m_o == 64) go(k_attn_kvq_tile<TY, HD, 1>);
+        else go(k_attn_kvq_tile<TY, HD, 2>);
+    } else if (p.m_p == 64) p.m_o == 16 ? go(k_attn_kvq_both<TY, HD, 1, 1>) : go(k_attn_kvq_both<TY, HD, 1, 2>);
+    else p.m_o == 16 ? go(k_attn_kvq_both<TY, HD, 2, 1>) : go(k_attn_kvq_both<TY, HD, 2, 2>);
 }
 
 }  // namespace orc
@@ -815,11 +856,11 @@ extern "C" int orc_attn_kvq(int type, const float* d_q, int ldq, int n_seq, int 
         (((uintptr_t)d_q | (uintptr_t)d_out | (uintptr_t)d_kc | (uintptr_t)d_vc | (uintptr_t)d_pk | (uintptr_t)d_pv |
           (uintptr_t)d_work) & 15))
         return set_error(ORC_E_INVALID, "attn_kvq: null or misaligned pointer");
-    const int64_t jobs = (int64_t)n_kv * p.cp * p.tiles_p + (int64_t)n_seq * n_kv * p.co * p.tiles_o;
-    if (jobs > 0xffffff00ll / 256 - 8) return set_error(ORC_E_INVALID, "attn_kvq: too many rows");
+    const int64_t jobs_p = (int64_t)n_kv * p.cp * p.tiles_p, jobs_o = (int64_t)n_seq * n_kv * p.co * p.tiles_o;
+    if (jobs_p + jobs_o > 0xffffff00ll / 256 - 16) return set_error(ORC_E_INVALID, "attn_kvq: too many rows");
     KaArgs a{d_q, ldq, n_seq, n_tok, n_heads, n_kv, n_heads / n_kv, (const uint8_t*)d_pk, (const uint8_t*)d_pv,
              (const uint8_t*)d_kc, (const uint8_t*)d_vc, prefix_len, prefix_ctx, ctx, d_pos, pos_off, pos_limit, d_out,
-             ldo, nullptr, nullptr, (int)p.rows, p.shared, p.tiles_p, p.cp, p.tiles_o, p.co, 0, 0};
+             ldo, nullptr, nullptr, (int)p.rows, p.shared, p.tiles_p, p.cp, p.tiles_o, p.co, (int)jobs_p, (int)jobs_o};
     if (bytes) {
         a.part_o = (float*)d_work;
         a.part_ml = (float2*)((uint8_t*)d_work + (size_t)p.slots() * p.rows * head_dim * 4);
