@@ -166,6 +166,16 @@ template <int TY, int HD> struct KaV {
                 sc[i] = *(const u32x4*)(blk + kvq_code_bytes(TY, HD) + i * 64 + (lane >> 4) * 16);
         }
     }
+    // Makes each register group one whole value here. Without it the compiler (ROCm 7.2) took parts of them for
+    // temporaries between keep() and the products, where the next block's load is conditional: wrong results.
+    __device__ __forceinline__ void pin() {
+#pragma unroll
+        for (int i = 0; i < kN; ++i) asm volatile("" : "+v"(r[i]));
+        if constexpr (TY != ORC_F16) {
+#pragma unroll
+            for (int i = 0; i < HD / 32; ++i) asm volatile("" : "+v"(sc[i]));
+        }
+    }
     // The rows from key `n` of the block on count as zeros (0 times whatever they hold would not): the bytes'
     // scales, or the halves themselves.
     __device__ __forceinline__ void keep(int n, int lane) {
@@ -319,11 +329,33 @@ template <int HD, int RT> struct KaStreamLds {
 template <int TY, int HD, int RT>
 __device__ __forceinline__ void ka_stream(const KaArgs& a, const KaJob& j, KaStreamLds<HD, RT>& sh) {
     constexpr int DT = HD / 16, KS = HD / 32, BB = kvq_block_bytes(TY, HD), M = 16 * RT;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = lane & 15, g = lane >> 4;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 15, g = lane >> 4;
     const bool direct = a.cp + a.co == 1;
     if (j.b0 >= j.b1 && !direct) return;
     const int nbp = (a.prefix + kKvBlock - 1) / kKvBlock;
 
+    const int first_own = j.seq < 0 ? 0 : min(j.start + j.r0 / a.group - j.seq * a.n_tok + 1, j.len);  // the least vis
+    const uint8_t* pk = a.pk + (size_t)j.kv * (a.pctx / kKvBlock) * BB;
+    const uint8_t* pv = a.pv + (size_t)j.kv * (a.pctx / kKvBlock) * BB;
+    const size_t own = ((size_t)max(j.seq, 0) * a.n_kv + j.kv) * (a.ctx / kKvBlock) * BB;
+    KaK<TY, HD> kr[4] = {};
+    KaV<TY, HD> vr = {};
+    uint32_t ks = 0;
+    auto load_k = [&](int b) {
+        const uint8_t* kb = b < nbp ? pk + (size_t)b * BB : a.kc + own + (size_t)(b - nbp) * BB;
+#pragma unroll
+        for (int t = 0; t < 4; ++t) kr[t].load(kb, t, lane);
+        if constexpr (TY != ORC_F16) ks = *(const uint32_t*)(kb + kvq_code_bytes(TY, HD) + ((HD == 128 ? g : g >> 1) * 16 + c) * 4);
+    };
+    auto load_v = [&](int b) { vr.load(b < nbp ? pv + (size_t)b * BB : a.vc + own + (size_t)(b - nbp) * BB, lane); };
+    // One row tile: a block's bytes are on their way while q is split and while the block before it is worked on. Two
+    // row tiles, or 128 fp16 dims (128 registers of bytes), leave no registers for that, and both together none for V
+    // before K is done with.
+    constexpr bool kWide = TY == ORC_F16 && HD == 128, kAhead = RT == 1 && !kWide, kLateV = RT > 1 && kWide;
+    if (kAhead && j.b0 + wave < j.b1) {
+        load_k(j.b0 + wave);
+        load_v(j.b0 + wave);
+    }
     KaQ<TY, HD> q[RT];
     KaRow st[RT];
     int vis[RT];  // own rows that the lane's query row sees
@@ -336,23 +368,14 @@ __device__ __forceinline__ void ka_stream(const KaArgs& a, const KaJob& j, KaStr
 #pragma unroll
         for (int d = 0; d < DT; ++d) o[r][d] = kq_f4{0.f, 0.f, 0.f, 0.f};
     }
-    const int first_own = j.seq < 0 ? 0 : min(j.start + j.r0 / a.group - j.seq * a.n_tok + 1, j.len);  // the least vis
-    const uint8_t* pk = a.pk + (size_t)j.kv * (a.pctx / kKvBlock) * BB;
-    const uint8_t* pv = a.pv + (size_t)j.kv * (a.pctx / kKvBlock) * BB;
-    const size_t own = ((size_t)max(j.seq, 0) * a.n_kv + j.kv) * (a.ctx / kKvBlock) * BB;
     const float minus = ka_minus();
     float sgn = 1.f;
     for (int b = j.b0 + wave; b < j.b1; b += kKaWaves) {
         const bool pre = b < nbp;
-        const uint8_t* kb = pre ? pk + (size_t)b * BB : a.kc + own + (size_t)(b - nbp) * BB;
-        const uint8_t* vb = pre ? pv + (size_t)b * BB : a.vc + own + (size_t)(b - nbp) * BB;
-        KaK<TY, HD> kr[4];
-        KaV<TY, HD> vr;
-        uint32_t ks = 0;
-#pragma unroll
-        for (int t = 0; t < 4; ++t) kr[t].load(kb, t, lane);
-        if constexpr (TY != ORC_F16) ks = *(const uint32_t*)(kb + kvq_code_bytes(TY, HD) + ((HD == 128 ? g : g >> 1) * 16 + c) * 4);
-        vr.load(vb, lane);
+        if (!kAhead) {
+            load_k(b);
+            if (!kLateV) load_v(b);
+        }
         const int key0 = (pre ? b : b - nbp) * kKvBlock, lim = (pre ? a.prefix : j.len) - key0;
         kq_f4 s[RT][4];
 #pragma unroll
@@ -372,6 +395,8 @@ __device__ __forceinline__ void ka_stream(const KaArgs& a, const KaJob& j, KaStr
                 s[r][t] = z;
             }
         }
+        if (kAhead && b + kKaWaves < j.b1) load_k(b + kKaWaves);
+        if (kLateV) load_v(b);
         if (lim < kKvBlock || (!pre && first_own - key0 < kKvBlock)) {
 #pragma unroll
             for (int r = 0; r < RT; ++r) {
@@ -384,6 +409,7 @@ __device__ __forceinline__ void ka_stream(const KaArgs& a, const KaJob& j, KaStr
             }
         }
         if (lim < kKvBlock) vr.keep(lim, lane);
+        vr.pin();
         sgn = -sgn;
         const uint32_t sign = sgn < 0.f ? 0x80008000u : 0u;
         u32x4 ph[RT][2], pl[RT][2];
@@ -404,6 +430,7 @@ __device__ __forceinline__ void ka_stream(const KaArgs& a, const KaJob& j, KaStr
                 for (int i = 0; i < 4; ++i) o[r][d][i] = __builtin_fmaf(o[r][d][i], beta[r], z[i]);
             }
         }
+        if (kAhead && b + kKaWaves < j.b1) load_v(b + kKaWaves);
     }
     // join the waves' sums
 #pragma unroll
@@ -543,18 +570,6 @@ __device__ __forceinline__ void ka_tile(const KaArgs& a, const KaJob& j, KaTileL
     const int nbp = (a.prefix + kKvBlock - 1) / kKvBlock;
     const int w0 = j.r0 + wave * 16 * RT;  // the wave's first row
 
-    KaQ<TY, HD> q[RT];
-    KaRow st[RT];
-    int vis[RT];
-    kq_f4 o[RT][DT];
-#pragma unroll
-    for (int r = 0; r < RT; ++r) {
-        const int row = w0 + r * 16 + c, tok = row / a.group, hg = row - tok * a.group;
-        q[r].load(a.q + (int64_t)tok * a.ldq + (size_t)(j.kv * a.group + hg) * HD, row < j.r1, g);
-        vis[r] = j.seq < 0 ? 0 : min(j.start + tok - j.seq * a.n_tok + 1, j.len);
-#pragma unroll
-        for (int d = 0; d < DT; ++d) o[r][d] = kq_f4{0.f, 0.f, 0.f, 0.f};
-    }
     // own rows that the wave's first and last row see
     const int first_own = j.seq < 0 ? 0 : min(j.start + w0 / a.group - j.seq * a.n_tok + 1, j.len);
     const int last_own = j.seq < 0 ? 0 : min(j.start + (min(w0 + 16 * RT, j.r1) - 1) / a.group - j.seq * a.n_tok + 1, j.len);
@@ -562,7 +577,7 @@ __device__ __forceinline__ void ka_tile(const KaArgs& a, const KaJob& j, KaTileL
     const uint8_t* pk = a.pk + (size_t)j.kv * (a.pctx / kKvBlock) * BB;
     const uint8_t* pv = a.pv + (size_t)j.kv * (a.pctx / kKvBlock) * BB;
     const size_t own = ((size_t)max(j.seq, 0) * a.n_kv + j.kv) * (a.ctx / kKvBlock) * BB;
-    KaStage<TY, HD> sg;
+    KaStage<TY, HD> sg = {};
     auto load = [&](int b) {
         const bool pre = b < nbp;
         sg.load(pre ? pk + (size_t)b * BB : a.kc + own + (size_t)(b - nbp) * BB,
@@ -575,8 +590,20 @@ __device__ __forceinline__ void ka_tile(const KaArgs& a, const KaJob& j, KaTileL
     };
     const float minus = ka_minus();
     float sgn = 1.f;
+    if (j.b0 < j.b1) load(j.b0);  // on its way while q is split
+    KaQ<TY, HD> q[RT];
+    KaRow st[RT];
+    int vis[RT];
+    kq_f4 o[RT][DT];
+#pragma unroll
+    for (int r = 0; r < RT; ++r) {
+        const int row = w0 + r * 16 + c, tok = row / a.group, hg = row - tok * a.group;
+        q[r].load(a.q + (int64_t)tok * a.ldq + (size_t)(j.kv * a.group + hg) * HD, row < j.r1, g);
+        vis[r] = j.seq < 0 ? 0 : min(j.start + tok - j.seq * a.n_tok + 1, j.len);
+#pragma unroll
+        for (int d = 0; d < DT; ++d) o[r][d] = kq_f4{0.f, 0.f, 0.f, 0.f};
+    }
     if (j.b0 < j.b1) {
-        load(j.b0);
         put(j.b0, 0);
         load(min(j.b0 + 1, j.b1 - 1));
     }
@@ -744,13 +771,20 @@ template <int HD, int W> __global__ __launch_bounds__(256) void k_attn_kvq_merge
     __syncthreads();
     if (live) {
         const float* po = a.part_o + (size_t)row * HD + lane * E;
-#pragma unroll 4
-        for (int c = wave % W; c < n; c += W) {
-            const float e = wt[sub][c];
-            if (e == 0.f) continue;
-            const float* p = po + (size_t)c * a.n_rows * HD;
+        const size_t step = (size_t)a.n_rows * HD;
+        for (int c0 = wave % W; c0 < n; c0 += W * 8) {  // eight loads at a time; what an unwritten chunk holds is dropped
+            float x[8][E], e[8];
 #pragma unroll
-            for (int i = 0; i < E; ++i) v[i] += e * p[i];
+            for (int u = 0; u < 8; ++u) {
+                const int c = c0 + u * W;
+                e[u] = c < n ? wt[sub][c] : 0.f;
+#pragma unroll
+                for (int i = 0; i < E; ++i) x[u][i] = po[(size_t)min(c, n - 1) * step + i];
+            }
+#pragma unroll
+            for (int u = 0; u < 8; ++u)
+#pragma unroll
+                for (int i = 0; i < E; ++i) v[i] += e[u] == 0.f ? 0.f : e[u] * x[u][i];
         }
     }
     if constexpr (W > 1) {
@@ -770,6 +804,8 @@ template <int HD, int W> __global__ __launch_bounds__(256) void k_attn_kvq_merge
 }
 
 // ── host ─────────────────────────────────────────────────────────────────────
+constexpr int kKaFill = 512;  // workgroups that fill the card: two on each CU
+
 struct KaPlan {
     bool shared;
     int m_p, m_o;  // rows of a workgroup: 16 or 32 (the waves share out the keys), 64 or 128 (they share the operands)
@@ -781,10 +817,13 @@ struct KaPlan {
 
 static int ka_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 
-// Chunks of nb key blocks for `base` workgroups' worth of row tiles: about two workgroups per CU, at least `least`
-// blocks each.
-static int ka_chunks(int64_t base, int nb, int least) {
-    return (int)std::max<int64_t>(1, std::min<int64_t>(512 / base, nb / least));
+// Chunks of nb key blocks for `base` workgroups' worth of row tiles: at most `most` workgroups, and four blocks each or
+// more, all of a length but the last; one where `one` blocks are no more work than a second launch.
+static int ka_chunks(int64_t base, int nb, int64_t most, int one) {
+    if (getenv("KA_ONE")) one = atoi(getenv("KA_ONE"));
+    if (nb <= one) return 1;
+    const int n = (int)std::max<int64_t>(1, std::min<int64_t>(most / base, (nb + 3) / 4));
+    return ka_div(nb, ka_div(nb, n));
 }
 
 static KaPlan ka_plan(int n_seq, int n_tok, int n_heads, int n_kv, int prefix_len, int pos_limit) {
@@ -792,19 +831,23 @@ static KaPlan ka_plan(int n_seq, int n_tok, int n_heads, int n_kv, int prefix_le
     const int64_t group = n_heads / n_kv, rows_o = n_tok * group, rows_p = n_seq * rows_o;
     p.rows = (size_t)n_seq * n_tok * n_heads;
     const int nbp = ka_div(prefix_len, kKvBlock), nbo = ka_div(pos_limit, kKvBlock);
-    static int e_min = getenv("KA_MIN") ? atoi(getenv("KA_MIN")) : 2, e_mins = getenv("KA_MINS") ? atoi(getenv("KA_MINS")) : 4;
     // with this many rows each, sequences gain nothing from common tiles
     p.shared = prefix_len > 0 && n_seq > 1 && rows_o < 128;
     if (p.shared) {
         p.m_p = rows_p <= 16 ? 16 : rows_p <= 32 ? 32 : n_kv * (int64_t)ka_div(rows_p, 128) * (nbp / 8) >= 512 ? 128 : 64;
         p.m_o = p.m_p <= 32 ? p.m_p : rows_o <= 16 ? 16 : rows_o <= 32 ? 32 : p.m_p;
-        p.tiles_p = ka_div(rows_p, p.m_p);
-        p.cp = ka_chunks((int64_t)n_kv * p.tiles_p, nbp, p.m_p <= 32 ? e_mins : e_min);
     } else
         p.m_o = rows_o <= 16 ? 16 : rows_o <= 32 ? 32 : (int64_t)n_seq * n_kv * ka_div(rows_o, 128) >= 1024 ? 128 : 64;
-    if (getenv("KA_MO")) p.m_o = atoi(getenv("KA_MO"));
     p.tiles_o = ka_div(rows_o, p.m_o);
-    p.co = ka_chunks((int64_t)n_seq * n_kv * p.tiles_o, p.shared ? nbo : nbp + nbo, p.m_o <= 32 ? e_mins : e_min);
+    const int64_t base_o = (int64_t)n_seq * n_kv * p.tiles_o;
+    p.co = ka_chunks(base_o, p.shared ? nbo : nbp + nbo, kKaFill, p.m_o <= 32 ? 12 : 4);
+    if (p.shared) {
+        p.tiles_p = ka_div(rows_p, p.m_p);
+        const int64_t base_p = (int64_t)n_kv * p.tiles_p;
+        // short prefix chunks share the card with the own jobs; beside long ones those are done in passing
+        const bool lng = nbp * base_p >= 16 * kKaFill;
+        p.cp = ka_chunks(base_p, nbp, lng ? kKaFill : std::max<int64_t>(kKaFill / 2, kKaFill - base_o * p.co), 4);
+    }
     return p;
 }
 

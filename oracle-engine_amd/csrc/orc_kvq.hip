@@ -8,6 +8,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 namespace orc {
 
@@ -16,17 +17,27 @@ struct RopeFreqs {
     double f[64];  // angle of one position, per pair
 };
 
-// (cos, sin) of pos f_i times the table's factor, formed in 64 bits: an angle
-// of 2^17 radians has 2^-7 left of a 24-bit mantissa, and sums of rounded
-// angles drift with the position.
-__global__ __launch_bounds__(256) void k_rope_table(float2* out, int64_t pos0, int64_t n, int pairs, RopeFreqs fr,
-                                                    double mul) {
-    const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (t >= n * pairs) return;
-    const int64_t p = t / pairs;
-    double s, c;
-    sincos((double)(pos0 + p) * fr.f[t - p * pairs], &s, &c);
-    out[t] = make_float2((float)(c * mul), (float)(s * mul));
+// (cos, sin) of pos f_i times the table's factor, formed in 64 bits: an angle of 2^17 radians has 2^-7 left of a
+// 24-bit mantissa, and sums of rounded angles drift with the position. A thread takes one pair at `steps` rows, `rows`
+// apart: the sine and cosine of the first row's angle and of the step's, then one complex product per row (their error,
+// 2^-52 a row, stays 2^20 below the result's last place), a tenth of the work of a sine for every entry. Neighbouring
+// threads hold neighbouring pairs, so a workgroup writes rows in a row.
+__global__ __launch_bounds__(256) void k_rope_table(float2* out, int64_t pos0, int64_t n, int pairs, int rows, int steps,
+                                                    RopeFreqs fr, double mul) {
+    const int r = threadIdx.x / pairs, i = threadIdx.x - r * pairs;
+    if (r >= rows) return;
+    int64_t p = (int64_t)blockIdx.x * rows * steps + r;
+    double s, c, ds, dc;
+    sincos((double)(pos0 + p) * fr.f[i], &s, &c);
+    sincos((double)rows * fr.f[i], &ds, &dc);
+    s *= mul;
+    c *= mul;
+    for (int k = 0; k < steps && p < n; ++k, p += rows) {
+        out[p * pairs + i] = make_float2((float)c, (float)s);
+        const double t = c * dc - s * ds;
+        s = s * dc + c * ds;
+        c = t;
+    }
 }
 
 // ── quantisation ─────────────────────────────────────────────────────────────
@@ -144,6 +155,286 @@ template <int TY, int HD> __global__ __launch_bounds__(256) void k_kvq_store(Sto
     }
 }
 
+// Prompts: a workgroup per 64-position block of one kv head's K or V, and workgroups of q vectors behind them.
+// K: a thread takes HD / 8 dims of one key and the ones HD / 2 further on, a rotate-half pair's two sides, so that the
+// row is read once; its codes are whole 16 or 8 byte pieces of the block, stored in order. V: rows go through LDS,
+// since a stored piece is one dim of 16 keys; pieces that hold rows of other calls are written byte by byte.
+constexpr int kStoreBlocks = 16;  // tokens of a sequence from which on a call takes whole blocks
+enum { kRotHalf, kRotPairs, kRotAny };  // whole heads half-split; pairs (2 i, 2 i + 1), or nothing rotated; the rest
+
+template <int TY, int HD> struct StoreLds {
+    float x[64][HD + 1];
+    float d[64][HD / 32 + 1];
+};
+
+__device__ __forceinline__ float kvq_clamp(float v, float lim, bool& bad) {
+    bad |= !(fabsf(v) < __builtin_inff());
+    return fminf(fmaxf(v, -lim), lim);  // of a NaN: lim, in a group that is marked
+}
+__device__ __forceinline__ _Float16 kvq_half(float y) {
+    if (fabsf(y) < __builtin_inff()) y = fminf(fmaxf(y, -65504.f), 65504.f);
+    return (_Float16)y;
+}
+
+template <int TY, int HD>
+__device__ __forceinline__ void kvq_store_k(const StoreArgs& a, int mode, int seq, int kv, int start, int64_t b) {
+    constexpr int P = HD / 8, L = HD / 4;
+    const int lane = threadIdx.x & 63, tile = threadIdx.x >> 6, c = lane & 15, u = lane >> 4;
+    const int64_t p = b * kKvBlock + tile * 16 + c, t = p - start;
+    const bool live = t >= 0 && t < a.n_tok;
+    float v[2][P] = {};
+    if (live) {
+        const float* x = a.qkv + ((int64_t)seq * a.n_tok + t) * a.ldqkv + (size_t)(a.n_heads + kv) * HD;
+        const float2* cs = a.rope + (a.rope_off + p) * (a.rot >> 1);
+        if (mode == kRotAny) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int e = 0; e < P; ++e) v[h][e] = kvq_rotated(x, h * (HD / 2) + u * P + e, ORC_ROPE_HALF, a.rot, cs);
+        } else {
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int e = 0; e < P; e += 4) {
+                    const kq_f4 w = *(const kq_f4*)(x + h * (HD / 2) + u * P + e);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) v[h][e + k] = w[k];
+                }
+            if (mode == kRotHalf) {
+#pragma unroll
+                for (int e = 0; e < P; ++e) {
+                    const float2 r = cs[u * P + e];
+                    const double va = v[0][e], vb = v[1][e], co = r.x, si = r.y;
+                    v[0][e] = (float)(va * co - vb * si);
+                    v[1][e] = (float)(va * si + vb * co);
+                }
+            } else {
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int e = 0; e < P; e += 2) {
+                        const int d = h * (HD / 2) + u * P + e;
+                        if (d < a.rot) {
+                            const float2 r = cs[d >> 1];
+                            const double va = v[h][e], vb = v[h][e + 1], co = r.x, si = r.y;
+                            v[h][e] = (float)(va * co - vb * si);
+                            v[h][e + 1] = (float)(va * si + vb * co);
+                        }
+                    }
+            }
+        }
+    }
+    uint8_t* blk = a.kc + (((size_t)seq * a.n_kv + kv) * (a.ctx / kKvBlock) + b) * kvq_block_bytes(TY, HD);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const int d0 = h * (HD / 2) + u * P, g = d0 / L, e0 = d0 % L;  // the operand's lane group, and where in its dims
+        if constexpr (TY == ORC_F16) {
+#pragma unroll
+            for (int e = 0; e < P; e += 8) {
+                kq_h8 y;
+#pragma unroll
+                for (int k = 0; k < 8; ++k) y[k] = kvq_half(v[h][e + k]);
+                if (live) *(kq_h8*)(blk + tile * 32 * HD + (e0 + e) / 8 * 1024 + (g * 16 + c) * 16) = y;
+            }
+        } else {
+            constexpr int M = kvq_levels(TY);
+            bool bad = false;
+            float mx = 0.f;
+#pragma unroll
+            for (int e = 0; e < P; ++e) {
+                v[h][e] = kvq_clamp(v[h][e], kKvMax, bad);
+                mx = fmaxf(mx, fabsf(v[h][e]));
+            }
+            int any = bad;
+#pragma unroll
+            for (int s = 16; s < 16 * (kKvGroup / P); s *= 2) {  // the threads of a scale group
+                mx = fmaxf(mx, __shfl_xor(mx, s, 64));
+                any |= __shfl_xor(any, s, 64);
+            }
+            const uint32_t byte = kvq_scale_byte<M>(mx);
+            const float D = kvq_scale(byte);
+            if (live && d0 % kKvGroup == 0)
+                blk[kvq_code_bytes(TY, HD) + d0 / kKvGroup * 64 + c * 4 + tile] = any ? 0xFF : byte;
+            uint32_t w[P / 4];
+#pragma unroll
+            for (int e = 0; e < P / 4; ++e) {
+                w[e] = 0;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) w[e] |= kvq_code<M>(v[h][e * 4 + k], D) << (8 * k);
+            }
+            if constexpr (TY == ORC_KV_Q8) {
+                uint8_t* at = blk + tile * 16 * HD + (g * 16 + c) * 16;
+                if (live) {
+                    if constexpr (HD == 128) *(u32x4*)(at + e0 / 16 * 1024) = u32x4{w[0], w[1], w[2], w[3]};
+                    else *(u32x2*)(at + e0) = u32x2{w[0], w[1]};
+                }
+            } else {  // the next thread group holds the upper halves
+#pragma unroll
+                for (int e = 0; e < P / 4; ++e) w[e] |= __shfl_xor(w[e], 16, 64) << 4;
+                uint8_t* at = blk + tile * 8 * HD + (g * 16 + c) * (L / 2);
+                if (live && !(u & 1)) {
+                    if constexpr (HD == 128) *(u32x4*)at = u32x4{w[0], w[1], w[2], w[3]};
+                    else *(u32x2*)at = u32x2{w[0], w[1]};
+                }
+            }
+        }
+    }
+}
+
+template <int TY, int HD>
+__device__ __forceinline__ void kvq_store_v(const StoreArgs& a, int seq, int kv, int start, int64_t b, StoreLds<TY, HD>& sh) {
+    const int tid = threadIdx.x;
+    const int64_t t0 = b * kKvBlock - start;  // token of the block's first row
+    const float* x = a.qkv + (int64_t)seq * a.n_tok * a.ldqkv + (size_t)(a.n_heads + a.n_kv + kv) * HD;
+    for (int it = tid; it < 64 * HD / 4; it += 256) {
+        const int r = it / (HD / 4), d = it % (HD / 4) * 4;
+        kq_f4 v = {0.f, 0.f, 0.f, 0.f};
+        if (t0 + r >= 0 && t0 + r < a.n_tok) v = *(const kq_f4*)(x + (t0 + r) * a.ldqkv + d);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) sh.x[r][d + k] = v[k];
+    }
+    __syncthreads();
+    uint8_t* blk = a.vc + (((size_t)seq * a.n_kv + kv) * (a.ctx / kKvBlock) + b) * kvq_block_bytes(TY, HD);
+    constexpr int M = kvq_levels(TY);
+    if constexpr (TY != ORC_F16) {
+        for (int it = tid; it < 64 * (HD / 32); it += 256) {
+            const int r = it & 63, grp = it >> 6;
+            bool bad = false;
+            float mx = 0.f;
+            for (int e = 0; e < 32; ++e) mx = fmaxf(mx, fabsf(kvq_clamp(sh.x[r][grp * 32 + e], kKvMax, bad)));
+            const uint32_t byte = kvq_scale_byte<M>(mx);
+            sh.d[r][grp] = kvq_scale(byte);
+            if (t0 + r >= 0 && t0 + r < a.n_tok) {
+                const int slot = (r >> 5) * 8 + ((r >> 4) & 1) * 4 + (r & 3);
+                blk[kvq_code_bytes(TY, HD) + grp * 64 + ((r & 15) >> 2) * 16 + slot] = bad ? 0xFF : byte;
+            }
+        }
+        __syncthreads();
+    }
+    constexpr int kUnits = TY == ORC_KV_Q4 ? HD * 2 : HD * 4;  // (dim or pair of dims, lane group)
+    for (int it = tid; it < kUnits; it += 256) {
+        const int lane = it & 63, dt = (it >> 6) * (TY == ORC_KV_Q4 ? 2 : 1), g = lane >> 4, d = dt * 16 + (lane & 15);
+        bool all = true;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) all &= t0 + q * 16 + g * 4 >= 0 && t0 + q * 16 + g * 4 + 3 < a.n_tok;
+        if constexpr (TY == ORC_F16) {
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                kq_h8 y;
+                _Float16* at = (_Float16*)(blk + dt * 2048 + s * 1024 + lane * 16);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) y[e] = kvq_half(sh.x[s * 32 + (e >> 2) * 16 + g * 4 + (e & 3)][d]);
+                if (all) *(kq_h8*)at = y;
+                else {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const int64_t t = t0 + s * 32 + (e >> 2) * 16 + g * 4 + (e & 3);
+                        if (t >= 0 && t < a.n_tok) at[e] = y[e];
+                    }
+                }
+            }
+        } else {
+            uint32_t w[4];
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const int r = (e >> 3) * 32 + ((e >> 2) & 1) * 16 + g * 4 + (e & 3);
+                bool bad = false;
+                uint32_t u = kvq_code<M>(kvq_clamp(sh.x[r][d], kKvMax, bad), sh.d[r][d >> 5]);
+                if constexpr (TY == ORC_KV_Q4) u |= kvq_code<M>(kvq_clamp(sh.x[r][d + 16], kKvMax, bad), sh.d[r][d >> 5]) << 4;
+                w[e >> 2] = (e & 3) ? w[e >> 2] | u << (8 * (e & 3)) : u;
+            }
+            uint8_t* at = blk + (TY == ORC_KV_Q4 ? dt >> 1 : dt) * 1024 + lane * 16;
+            if (all) *(u32x4*)at = u32x4{w[0], w[1], w[2], w[3]};
+            else {
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    const int64_t t = t0 + (e >> 3) * 32 + ((e >> 2) & 1) * 16 + g * 4 + (e & 3);
+                    if (t >= 0 && t < a.n_tok) at[e] = w[e >> 2] >> (8 * (e & 3));
+                }
+            }
+        }
+    }
+}
+
+// eight values of a q vector a thread: four and the four HD / 2 further on, or eight in a row
+template <int HD> __device__ __forceinline__ void kvq_store_q(const StoreArgs& a, int mode, int64_t it) {
+    const int part = (int)(it % (HD / 8));
+    const int64_t hv = it / (HD / 8), row = hv / a.n_heads;
+    if (row >= (int64_t)a.n_seq * a.n_tok) return;
+    const int h = (int)(hv - row * a.n_heads), seq = (int)(row / a.n_tok);
+    const int start = kvq_start(a.d_pos, seq, a.pos_off, a.ctx);
+    const int64_t p = start + (row - (int64_t)seq * a.n_tok);
+    if (start < 0 || p >= a.ctx) return;
+    const float* x = a.qkv + row * a.ldqkv + (size_t)h * HD;
+    float* q = a.q + row * a.ldq + (size_t)h * HD;
+    const float2* cs = a.rope + (a.rope_off + p) * (a.rot >> 1);
+    const int d0 = mode == kRotPairs ? part * 8 : part * 4, d1 = mode == kRotPairs ? d0 + 4 : d0 + HD / 2;
+    kq_f4 v0 = *(const kq_f4*)(x + d0), v1 = *(const kq_f4*)(x + d1);
+    if (mode == kRotHalf) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const float2 r = cs[d0 + e];
+            const double va = v0[e], vb = v1[e], co = r.x, si = r.y;
+            v0[e] = (float)(va * co - vb * si);
+            v1[e] = (float)(va * si + vb * co);
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; e += 2) {
+            if (d0 + e < a.rot) {
+                const float2 r = cs[(d0 + e) >> 1];
+                const double va = v0[e], vb = v0[e + 1], co = r.x, si = r.y;
+                v0[e] = (float)(va * co - vb * si);
+                v0[e + 1] = (float)(va * si + vb * co);
+            }
+            if (d1 + e < a.rot) {
+                const float2 r = cs[(d1 + e) >> 1];
+                const double va = v1[e], vb = v1[e + 1], co = r.x, si = r.y;
+                v1[e] = (float)(va * co - vb * si);
+                v1[e + 1] = (float)(va * si + vb * co);
+            }
+        }
+    }
+    *(kq_f4*)(q + d0) = v0;
+    *(kq_f4*)(q + d1) = v1;
+}
+
+// Grid: blocks_kv workgroups of K and V blocks (nblk a sequence and head), then q. kRotAny's q vectors, whose pairs lie
+// anywhere in the head, take a wave each as in k_kvq_store.
+template <int TY, int HD>
+__global__ __launch_bounds__(256) void k_kvq_store_blocks(StoreArgs a, int mode, int nblk, int64_t blocks_kv) {
+    __shared__ StoreLds<TY, HD> sh;
+    int64_t w = blockIdx.x;
+    if (w < blocks_kv) {
+        const int bi = (int)(w % nblk), kv2 = (int)(w / nblk % (2 * a.n_kv)), seq = (int)(w / nblk / (2 * a.n_kv));
+        const int start = kvq_start(a.d_pos, seq, a.pos_off, a.ctx);
+        const int64_t b = start / kKvBlock + (int64_t)bi;
+        if (start < 0 || b >= a.ctx / kKvBlock || b * kKvBlock >= (int64_t)start + a.n_tok) return;
+        if (kv2 < a.n_kv) kvq_store_k<TY, HD>(a, mode, seq, kv2, start, b);
+        else kvq_store_v<TY, HD>(a, seq, kv2 - a.n_kv, start, b, sh);
+        return;
+    }
+    w -= blocks_kv;
+    if (mode != kRotAny) {
+        kvq_store_q<HD>(a, mode, w * 256 + threadIdx.x);
+        return;
+    }
+    const int lane = threadIdx.x & 63;
+    const int64_t hv = w * 4 + (threadIdx.x >> 6), row = hv / a.n_heads;
+    if (row >= (int64_t)a.n_seq * a.n_tok) return;
+    const int h = (int)(hv - row * a.n_heads), seq = (int)(row / a.n_tok);
+    const int start = kvq_start(a.d_pos, seq, a.pos_off, a.ctx);
+    const int64_t p = start + (row - (int64_t)seq * a.n_tok);
+    if (start < 0 || p >= a.ctx) return;
+    const float* x = a.qkv + row * a.ldqkv + (size_t)h * HD;
+    float* q = a.q + row * a.ldq + (size_t)h * HD;
+    float v[HD / 64];
+#pragma unroll
+    for (int e = 0; e < HD / 64; ++e) v[e] = kvq_rotated(x, lane + 64 * e, a.layout, a.rot, a.rope + (a.rope_off + p) * (a.rot >> 1));
+#pragma unroll
+    for (int e = 0; e < HD / 64; ++e) q[lane + 64 * e] = v[e];
+}
+
 // ── read-back ────────────────────────────────────────────────────────────────
 template <int TY, int HD> __global__ __launch_bounds__(256) void k_kvq_load(const uint8_t* kc, const uint8_t* vc,
                                                                             int n_kv, int ctx, const int32_t* d_pos,
@@ -168,6 +459,90 @@ template <int TY, int HD> __global__ __launch_bounds__(256) void k_kvq_load(cons
         }
     }
     (is_v ? vo : ko)[((size_t)blockIdx.y * n + j) * HD + d] = y;
+}
+
+// Many rows: a workgroup per 64-position block of one head's K or V. Codes are loaded as the whole pieces they are
+// stored in, values turned into rows in LDS, and rows stored in order.
+template <int TY, int HD> __global__ __launch_bounds__(256) void k_kvq_load_blocks(const uint8_t* kc, const uint8_t* vc,
+                                                                                   int n_kv, int ctx, const int32_t* d_pos,
+                                                                                   int pos_off, int n, float* ko, float* vo) {
+    constexpr int BB = kvq_block_bytes(TY, HD), CB = kvq_code_bytes(TY, HD), L = HD / 4;
+    __shared__ float sh[kKvBlock][HD + 4];
+    const int tid = threadIdx.x, seq = blockIdx.y / n_kv;
+    const bool is_v = blockIdx.z == (ko ? 1 : 0);
+    const int64_t start = (int64_t)(d_pos ? d_pos[seq] : 0) + pos_off, b = (start >> 6) + blockIdx.x;
+    const int64_t j0 = b * kKvBlock - start;  // output row of the block's first one
+    if (j0 >= n) return;
+    float* out = (is_v ? vo : ko) + (size_t)blockIdx.y * n * HD;
+    const bool in = b >= 0 && b < ctx / kKvBlock;
+    if (in) {
+        const uint8_t* blk = (is_v ? vc : kc) + ((size_t)blockIdx.y * (ctx / kKvBlock) + b) * BB;
+        const int lane = tid & 63, c = lane & 15, g = lane >> 4;
+        constexpr float bias = kvq_levels(TY) + 1;
+        if (!is_v) {  // a wave takes a tile of 16 keys
+            const int tile = tid >> 6;
+            float s = 0.f;
+            if constexpr (TY != ORC_F16) s = kvq_scale(blk[CB + (g * L / kKvGroup) * 64 + c * 4 + tile]) * 0.0625f;
+            float* row = &sh[tile * 16 + c][g * L];
+            constexpr int kP = TY == ORC_F16 ? 8 : L < 16 ? L : 16;  // values of a piece (4 bits: all)
+            if constexpr (TY == ORC_F16) {
+#pragma unroll
+                for (int e = 0; e < L; e += kP) {
+                    const kq_h8 h = *(const kq_h8*)(blk + tile * 32 * HD + e / 8 * 1024 + lane * 16);
+#pragma unroll
+                    for (int k = 0; k < 8; k += 4) *(kq_f4*)(row + e + k) = kq_f4{(float)h[k], (float)h[k + 1], (float)h[k + 2], (float)h[k + 3]};
+                }
+            } else if constexpr (TY == ORC_KV_Q8) {
+#pragma unroll
+                for (int e = 0; e < L; e += 16) {
+                    const u32x4 w = *(const u32x4*)(blk + tile * 16 * HD + e / 16 * 1024 + lane * 16);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        *(kq_f4*)(row + e + k * 4) = kq_f4{(ubyte_f(w[k], 0) - bias) * s, (ubyte_f(w[k], 1) - bias) * s,
+                                                           (ubyte_f(w[k], 2) - bias) * s, (ubyte_f(w[k], 3) - bias) * s};
+                }
+            } else {
+                const uint8_t* at = blk + tile * 8 * HD + lane * (L / 2);
+#pragma unroll
+                for (int k = 0; k < L / 8; ++k) {
+                    const uint32_t w = *(const uint32_t*)(at + k * 4), lo = w & 0x0F0F0F0Fu, hi = (w >> 4) & 0x0F0F0F0Fu;
+                    *(kq_f4*)(row + k * 4) = kq_f4{(ubyte_f(lo, 0) - bias) * s, (ubyte_f(lo, 1) - bias) * s,
+                                                   (ubyte_f(lo, 2) - bias) * s, (ubyte_f(lo, 3) - bias) * s};
+                    *(kq_f4*)(row + L / 2 + k * 4) = kq_f4{(ubyte_f(hi, 0) - bias) * s, (ubyte_f(hi, 1) - bias) * s,
+                                                           (ubyte_f(hi, 2) - bias) * s, (ubyte_f(hi, 3) - bias) * s};
+                }
+            }
+        } else {  // a wave takes every fourth dim tile
+            for (int dt = tid >> 6; dt < HD / 16; dt += 4) {
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {  // (step, half): four keys
+                    float v[4];
+                    if constexpr (TY == ORC_F16) {
+                        typedef _Float16 h4 __attribute__((ext_vector_type(4)));
+                        const h4 h = *(const h4*)(blk + dt * 2048 + (q >> 1) * 1024 + lane * 16 + (q & 1) * 8);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) v[i] = (float)h[i];
+                    } else {
+                        uint32_t w = *(const uint32_t*)(blk + (TY == ORC_KV_Q4 ? dt >> 1 : dt) * 1024 + lane * 16 + q * 4);
+                        if constexpr (TY == ORC_KV_Q4) w = (w >> (dt & 1) * 4) & 0x0F0F0F0Fu;
+                        const uint32_t s = *(const uint32_t*)(blk + CB + (dt >> 1) * 64 + g * 16 + q * 4);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) v[i] = (ubyte_f(w, i) - bias) * (kvq_scale((s >> (8 * i)) & 0xFF) * 0.0625f);
+                    }
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) sh[q * 16 + g * 4 + i][dt * 16 + c] = v[i];
+                }
+            }
+        }
+    }
+    __syncthreads();
+    for (int it = tid; it < kKvBlock * HD / 4; it += 256) {
+        const int r = it / (HD / 4), d = it % (HD / 4) * 4;
+        if (j0 + r < 0 || j0 + r >= n) continue;
+        kq_f4 y = {0.f, 0.f, 0.f, 0.f};
+        if (in) y = *(const kq_f4*)&sh[r][d];
+        *(kq_f4*)(out + (j0 + r) * HD + d) = y;
+    }
 }
 
 }  // namespace orc
@@ -221,10 +596,13 @@ extern "C" int orc_rope_table(float* d_rope, int pos0, int n_pos, int rot_dim, d
         fr.f[i] = f;
     }
     if (!n_pos) return ORC_OK;
-    const int64_t total = (int64_t)n_pos * (rot_dim / 2);
-    if (total > 0xffffff00ll) return set_error(ORC_E_INVALID, "rope_table: more than 2^32 pairs");
-    hipLaunchKernelGGL(k_rope_table, dim3((unsigned)((total + 255) / 256)), dim3(256), 0, resolve_stream(s),
-                       (float2*)d_rope, (int64_t)pos0, (int64_t)n_pos, rot_dim / 2, fr, mul);
+    const int pairs = rot_dim / 2, rows = 256 / pairs;
+    // 16 rows a thread where that still makes two workgroups for every CU, else 4
+    const int steps = n_pos / (rows * 16) >= 512 ? 16 : 4;
+    const int64_t blocks = ((int64_t)n_pos + rows * steps - 1) / (rows * steps);
+    if (blocks > 0xffffff00ll / 256) return set_error(ORC_E_INVALID, "rope_table: too many positions");
+    hipLaunchKernelGGL(k_rope_table, dim3((unsigned)blocks), dim3(256), 0, resolve_stream(s), (float2*)d_rope, (int64_t)pos0,
+                       (int64_t)n_pos, pairs, rows, steps, fr, mul);
     ORC_LAUNCH_CHECK();
     return ORC_OK;
 }
@@ -252,11 +630,29 @@ extern "C" int orc_kvq_store(int type, const float* d_qkv, int ldqkv, int n_seq,
     if (blocks > 0xffffff00ll / 256) return set_error(ORC_E_INVALID, "kvq_store: too many rows");
     const StoreArgs a{d_qkv, ldqkv, n_seq, n_tok, n_heads, n_kv, rope_layout, rot_dim, (const float2*)d_rope, rope_off,
                       d_pos, pos_off, d_q, ldq, (uint8_t*)d_kc, (uint8_t*)d_vc, ctx};
-    auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(256), 0, resolve_stream(s), a); };
-    if (head_dim == 64)
-        type == ORC_F16 ? go(k_kvq_store<ORC_F16, 64>) : type == ORC_KV_Q8 ? go(k_kvq_store<ORC_KV_Q8, 64>) : go(k_kvq_store<ORC_KV_Q4, 64>);
-    else
-        type == ORC_F16 ? go(k_kvq_store<ORC_F16, 128>) : type == ORC_KV_Q8 ? go(k_kvq_store<ORC_KV_Q8, 128>) : go(k_kvq_store<ORC_KV_Q4, 128>);
+    const hipStream_t st = resolve_stream(s);
+    auto each = [&](auto f) {  // f of (type, head size)
+        using std::integral_constant;
+        auto with = [&](auto ty) { head_dim == 64 ? f(ty, integral_constant<int, 64>()) : f(ty, integral_constant<int, 128>()); };
+        if (type == ORC_F16) with(integral_constant<int, ORC_F16>());
+        else if (type == ORC_KV_Q8) with(integral_constant<int, ORC_KV_Q8>());
+        else with(integral_constant<int, ORC_KV_Q4>());
+    };
+    if (n_tok < kStoreBlocks)
+        each([&](auto ty, auto hd) {
+            hipLaunchKernelGGL((k_kvq_store<decltype(ty)::value, decltype(hd)::value>), dim3((unsigned)blocks), dim3(256), 0, st, a);
+        });
+    else {
+        const int mode = rope_layout == ORC_ROPE_PAIRS || !rot_dim ? kRotPairs : rot_dim == head_dim ? kRotHalf : kRotAny;
+        const int nblk = (n_tok + 2 * kKvBlock - 2) / kKvBlock;  // blocks that n_tok rows may touch
+        const int64_t kv = (int64_t)n_seq * 2 * n_kv * nblk, q = (int64_t)n_seq * n_tok * n_heads;
+        const int64_t all = kv + (mode == kRotAny ? (q + 3) / 4 : (q * (head_dim / 8) + 255) / 256);
+        if (all > 0xffffff00ll / 256) return set_error(ORC_E_INVALID, "kvq_store: too many rows");
+        each([&](auto ty, auto hd) {
+            hipLaunchKernelGGL((k_kvq_store_blocks<decltype(ty)::value, decltype(hd)::value>), dim3((unsigned)all), dim3(256), 0, st,
+                               a, mode, nblk, kv);
+        });
+    }
     ORC_LAUNCH_CHECK();
     return ORC_OK;
 }
@@ -275,18 +671,23 @@ extern "C" int orc_kvq_load(int type, const void* d_kc, const void* d_vc, int n_
         return set_error(ORC_E_INVALID, "kvq_load: rows must lie in the cache");
     const int z = (d_k ? 1 : 0) + (d_v ? 1 : 0);
     if (!n_seq || !n || !z) return ORC_OK;
-    const int64_t blocks = ((int64_t)n * head_dim + 255) / 256;
-    if (blocks > 0xffffff00ll / 256) return set_error(ORC_E_INVALID, "kvq_load: too many rows");
     if ((int64_t)n_seq * n_kv > 65535) return set_error(ORC_E_INVALID, "kvq_load: more than 65535 sequence heads");
+    const bool many = n >= kStoreBlocks;
+    const int64_t blocks = many ? ((int64_t)n + 2 * kKvBlock - 2) / kKvBlock : ((int64_t)n * head_dim + 255) / 256;
+    if (blocks > 0xffffff00ll / 256) return set_error(ORC_E_INVALID, "kvq_load: too many rows");
     const dim3 grid((unsigned)blocks, (unsigned)(n_seq * n_kv), (unsigned)z);
     auto go = [&](auto kernel) {
         hipLaunchKernelGGL(kernel, grid, dim3(256), 0, resolve_stream(s), (const uint8_t*)d_kc, (const uint8_t*)d_vc, n_kv,
                            ctx, d_pos, pos_off, n, d_k, d_v);
     };
-    if (head_dim == 64)
-        type == ORC_F16 ? go(k_kvq_load<ORC_F16, 64>) : type == ORC_KV_Q8 ? go(k_kvq_load<ORC_KV_Q8, 64>) : go(k_kvq_load<ORC_KV_Q4, 64>);
-    else
-        type == ORC_F16 ? go(k_kvq_load<ORC_F16, 128>) : type == ORC_KV_Q8 ? go(k_kvq_load<ORC_KV_Q8, 128>) : go(k_kvq_load<ORC_KV_Q4, 128>);
+    auto with = [&](auto ty) {
+        constexpr int T = decltype(ty)::value;
+        if (many) head_dim == 64 ? go(k_kvq_load_blocks<T, 64>) : go(k_kvq_load_blocks<T, 128>);
+        else head_dim == 64 ? go(k_kvq_load<T, 64>) : go(k_kvq_load<T, 128>);
+    };
+    if (type == ORC_F16) with(std::integral_constant<int, ORC_F16>());
+    else if (type == ORC_KV_Q8) with(std::integral_constant<int, ORC_KV_Q8>());
+    else with(std::integral_constant<int, ORC_KV_Q4>());
     ORC_LAUNCH_CHECK();
     return ORC_OK;
 }

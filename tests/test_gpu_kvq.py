@@ -97,7 +97,8 @@ def _same(a, b):
 STORES = [(1, 1, 2, 1, 64, [0], orc.ROPE_HALF, None), (1, 1, 14, 2, 128, [63], orc.ROPE_PAIRS, None),
           (3, 1, 4, 2, 192, [64, -1, 191], orc.ROPE_HALF, 32), (2, 5, 3, 3, 128, [61, 125], orc.ROPE_PAIRS, 6),
           (1, 130, 4, 1, 192, [7], orc.ROPE_HALF, 58), (2, 64, 2, 2, 256, [0, 100], orc.ROPE_PAIRS, 0),
-          (2, 200, 1, 2, 256, [64, -3], orc.ROPE_HALF, None)]
+          (2, 200, 1, 2, 256, [64, -3], orc.ROPE_HALF, None), (1, 70, 3, 2, 128, [30], orc.ROPE_PAIRS, 34),
+          (3, 16, 2, 1, 64, [48, 49, 3], orc.ROPE_PAIRS, None), (1, 15, 5, 1, 64, [50], orc.ROPE_HALF, 20)]
 
 
 @pytest.mark.parametrize("ty", TYPES)
@@ -175,7 +176,11 @@ def test_values_at_the_borders_of_the_formats(dev, ty, hd):
     qkv = np.concatenate([rng.normal(0, 1, (n, hd)).astype(np.float32), x.reshape(n, -1), x[::-1].reshape(n, -1)], 1)
     c = Caches(dev, ty, 1, KV, 64, hd)
     c.store(qkv, n, 1)
+    few = Caches(dev, ty, 1, KV, 64, hd)  # the same rows by calls of a few tokens each: the same values
+    for a in range(0, n, 9):
+        few.store(qkv[a:a + 9], min(9, n - a), 1, off=a)
     k, v = c.load(64)
+    assert all(_same(p, q) for p, q in zip(few.load(64), (k, v)))
     want = ref.quantised(ty, x)
     assert _same(k[0].transpose(1, 0, 2), want) and _same(v[0].transpose(1, 0, 2), want[::-1])
 
