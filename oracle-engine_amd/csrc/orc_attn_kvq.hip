@@ -20,7 +20,15 @@
 
 namespace orc {
 
-constexpr int kKaWaves = 4;
+// Division of a non-negative int by one that the host knows: a product and a shift instead of the 40 instructions of a
+// quotient of two registers, which stood between a workgroup's start and its first load.
+struct KaDiv {
+    uint32_t mul;  // 2^(31 + shift) / d rounded down, and 1
+    int shift, d;
+    __device__ __forceinline__ int operator()(int n) const {
+        return d == 1 ? n : (int)(__umulhi((uint32_t)n << 1, mul) >> shift);
+    }
+};
 
 struct KaArgs {
     const float* q;
@@ -37,11 +45,12 @@ struct KaArgs {
     // jobs: prefix ones (shared form only), then own ones
     int shared, tiles_p, cp, tiles_o, co;
     int jobs_p, jobs_o;
+    KaDiv by_group, by_kv, by_tiles_p, by_cp, by_tiles_o, by_co, by_heads, by_tok;
 };
 
 // Blocks [b0, b1) of chunk c of n chunks over nb blocks.
-__device__ __forceinline__ void ka_chunk(int nb, int n, int c, int& b0, int& b1) {
-    const int per = (nb + n - 1) / n;
+__device__ __forceinline__ void ka_chunk(int nb, const KaDiv& n, int c, int& b0, int& b1) {
+    const int per = n(nb + n.d - 1);
     b0 = min(nb, c * per);
     b1 = min(nb, b0 + per);
 }
@@ -53,43 +62,51 @@ struct KaJob {
     int kv, seq, r0, r1, b0, b1, slot, start, len;
 };
 
-__device__ __forceinline__ bool ka_job(const KaArgs& a, int m_p, int m_o, KaJob& j) {
+// The rows, from the grid alone.
+__device__ __forceinline__ bool ka_rows(const KaArgs& a, int m_p, int m_o, KaJob& j) {
     // Every XCD takes an eighth of the prefix jobs, then an eighth of the own ones, each in order: the row tiles of one
     // chunk, which read the same keys, share its L2.
     const int per_p = (a.jobs_p + 7) / 8, per_o = (a.jobs_o + 7) / 8, x = blockIdx.x & 7, i = blockIdx.x >> 3;
     const bool pre = i < per_p;
-    int w = pre ? x * per_p + i : x * per_o + i - per_p;
+    const int w = pre ? x * per_p + i : x * per_o + i - per_p;
     if (w >= (pre ? a.jobs_p : a.jobs_o)) return false;
-    const int nbp = (a.prefix + kKvBlock - 1) / kKvBlock;
     if (pre) {
-        const int tile = w % a.tiles_p, c = w / a.tiles_p % a.cp;
-        j.kv = w / a.tiles_p / a.cp;
+        const int t = a.by_tiles_p(w), tile = w - t * a.tiles_p;
+        j.kv = a.by_cp(t);
+        j.slot = t - j.kv * a.cp;
         j.seq = -1;
         j.r0 = tile * m_p;
         j.r1 = min(j.r0 + m_p, a.n_seq * a.n_tok * a.group);
-        j.start = j.len = 0;
-        j.slot = c;
-        ka_chunk(nbp, a.cp, c, j.b0, j.b1);
         return true;
     }
-    const int tile = a.tiles_o - 1 - w % a.tiles_o, c = w / a.tiles_o % a.co;  // the longest rows first
-    const int sk = w / a.tiles_o / a.co, rows = a.n_tok * a.group;
-    j.seq = sk / a.n_kv;
-    j.kv = sk % a.n_kv;
+    const int t = a.by_tiles_o(w), tile = (t + 1) * a.tiles_o - 1 - w;  // the longest rows first
+    const int sk = a.by_co(t), rows = a.n_tok * a.group;
+    j.slot = a.cp + t - sk * a.co;
+    j.seq = a.by_kv(sk);
+    j.kv = sk - j.seq * a.n_kv;
     j.r0 = j.seq * rows + tile * m_o;
     j.r1 = min(j.r0 + m_o, (j.seq + 1) * rows);
+    return true;
+}
+
+// The keys, which may depend on a position in device memory.
+__device__ __forceinline__ void ka_keys(const KaArgs& a, KaJob& j) {
+    const int nbp = (a.prefix + kKvBlock - 1) / kKvBlock;
+    if (j.seq < 0) {
+        j.start = j.len = 0;
+        ka_chunk(nbp, a.by_cp, j.slot, j.b0, j.b1);
+        return;
+    }
     j.start = kvq_start(a.d_pos, j.seq, a.pos_off, a.limit);
     j.len = j.start < 0 ? 0 : (int)min((int64_t)j.start + a.n_tok, (int64_t)a.limit);
-    j.slot = a.cp + c;
     const int first = a.shared ? nbp : 0;
     const int nb = j.len ? nbp - first + (j.len + kKvBlock - 1) / kKvBlock : 0;
-    ka_chunk(nb, a.co, c, j.b0, j.b1);
+    ka_chunk(nb, a.by_co, j.slot - a.cp, j.b0, j.b1);
     j.b0 += first;
     j.b1 += first;
     // nothing behind the tile's last token
-    const int last = min(j.start + (j.r1 - 1) / a.group - j.seq * a.n_tok, j.len - 1);
+    const int last = min(j.start + a.by_group(j.r1 - 1) - j.seq * a.n_tok, j.len - 1);
     if (j.len) j.b1 = min(j.b1, nbp + last / kKvBlock + 1);
-    return true;
 }
 
 // ── operands ─────────────────────────────────────────────────────────────────
@@ -238,22 +255,22 @@ __device__ __forceinline__ float ka_minus() {
 
 // A query row as operands: its head dims (hd / 4 per lane group) times a power
 // of two that brings the largest below 2^15, in two halves; f turns its scores into powers of two.
+template <int HD> struct KaRaw {
+    kq_f4 v[HD / 16];
+    __device__ __forceinline__ void load(const float* p, int g) {
+#pragma unroll
+        for (int i = 0; i < HD / 16; ++i) v[i] = *(const kq_f4*)(p + g * (HD / 4) + i * 4);
+    }
+};
 template <int TY, int HD> struct KaQ {
     kq_h8 hi[HD / 32], lo[HD / 32];
     float f;
-    __device__ __forceinline__ void load(const float* p, bool live, int g) {
-        float v[HD / 4];
+    __device__ __forceinline__ void split(const KaRaw<HD>& x) {
         float mx = 0.f;
 #pragma unroll
-        for (int i = 0; i < HD / 16; ++i) {
-            kq_f4 t = {0.f, 0.f, 0.f, 0.f};
-            if (live) t = *(const kq_f4*)(p + g * (HD / 4) + i * 4);
+        for (int i = 0; i < HD / 16; ++i)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                v[i * 4 + e] = t[e];
-                mx = fmaxf(mx, fabsf(t[e]));
-            }
-        }
+            for (int e = 0; e < 4; ++e) mx = fmaxf(mx, fabsf(x.v[i][e]));
         mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
         mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
         int ex = 0;
@@ -265,7 +282,7 @@ template <int TY, int HD> struct KaQ {
             uint32_t h[4], l[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-                h[e] = ka_split(ldexpf(v[j * 8 + 2 * e], ex), ldexpf(v[j * 8 + 2 * e + 1], ex), -1.f, l[e]);
+                h[e] = ka_split(ldexpf(x.v[j * 2 + e / 2][e % 2 * 2], ex), ldexpf(x.v[j * 2 + e / 2][e % 2 * 2 + 1], ex), -1.f, l[e]);
             hi[j] = __builtin_bit_cast(kq_h8, u32x4{h[0], h[1], h[2], h[3]});
             lo[j] = __builtin_bit_cast(kq_h8, u32x4{l[0], l[1], l[2], l[3]});
         }
@@ -319,22 +336,29 @@ struct KaRow {
 };
 
 // ── few rows: the waves share out the keys ───────────────────────────────────
-// A workgroup takes 16 RT rows; its waves take every fourth key block each,
+// A workgroup takes 16 RT rows; its NW waves take every NW-th key block each,
 // straight from memory to operands, and join their sums at the end.
-template <int HD, int RT> struct KaStreamLds {
-    float o[kKaWaves][16 * RT][HD + 4];
-    float2 ml[kKaWaves][16 * RT];
+template <int HD, int RT, int NW> struct KaStreamLds {
+    float o[NW][16 * RT][HD + 4];
+    float2 ml[NW][16 * RT];
 };
 
-template <int TY, int HD, int RT>
-__device__ __forceinline__ void ka_stream(const KaArgs& a, const KaJob& j, KaStreamLds<HD, RT>& sh) {
+template <int TY, int HD, int RT, int NW>
+__device__ __forceinline__ void ka_stream(const KaArgs& a, KaJob j, KaStreamLds<HD, RT, NW>& sh) {
     constexpr int DT = HD / 16, KS = HD / 32, BB = kvq_block_bytes(TY, HD), M = 16 * RT;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 15, g = lane >> 4;
+    KaRaw<HD> raw[RT];  // asked for before the position that the keys depend on is there
+#pragma unroll
+    for (int r = 0; r < RT; ++r) {
+        const int row = min(j.r0 + r * 16 + c, j.r1 - 1), tok = a.by_group(row), hg = row - tok * a.group;
+        raw[r].load(a.q + (int64_t)tok * a.ldq + (size_t)(j.kv * a.group + hg) * HD, g);
+    }
+    ka_keys(a, j);
     const bool direct = a.cp + a.co == 1;
     if (j.b0 >= j.b1 && !direct) return;
     const int nbp = (a.prefix + kKvBlock - 1) / kKvBlock;
 
-    const int first_own = j.seq < 0 ? 0 : min(j.start + j.r0 / a.group - j.seq * a.n_tok + 1, j.len);  // the least vis
+    const int first_own = j.seq < 0 ? 0 : min(j.start + a.by_group(j.r0) - j.seq * a.n_tok + 1, j.len);  // the least vis
     const uint8_t* pk = a.pk + (size_t)j.kv * (a.pctx / kKvBlock) * BB;
     const uint8_t* pv = a.pv + (size_t)j.kv * (a.pctx / kKvBlock) * BB;
     const size_t own = ((size_t)max(j.seq, 0) * a.n_kv + j.kv) * (a.ctx / kKvBlock) * BB;
@@ -362,15 +386,15 @@ __device__ __forceinline__ void ka_stream(const KaArgs& a, const KaJob& j, KaStr
     kq_f4 o[RT][DT];
 #pragma unroll
     for (int r = 0; r < RT; ++r) {
-        const int row = j.r0 + r * 16 + c, tok = row / a.group, hg = row - tok * a.group;
-        q[r].load(a.q + (int64_t)tok * a.ldq + (size_t)(j.kv * a.group + hg) * HD, row < j.r1, g);
+        const int tok = a.by_group(min(j.r0 + r * 16 + c, j.r1 - 1));
+        q[r].split(raw[r]);
         vis[r] = j.seq < 0 ? 0 : min(j.start + tok - j.seq * a.n_tok + 1, j.len);
 #pragma unroll
         for (int d = 0; d < DT; ++d) o[r][d] = kq_f4{0.f, 0.f, 0.f, 0.f};
     }
     const float minus = ka_minus();
     float sgn = 1.f;
-    for (int b = j.b0 + wave; b < j.b1; b += kKaWaves) {
+    for (int b = j.b0 + wave; b < j.b1; b += NW) {
         const bool pre = b < nbp;
         if (!kAhead) {
             load_k(b);
@@ -395,7 +419,7 @@ __device__ __forceinline__ void ka_stream(const KaArgs& a, const KaJob& j, KaStr
                 s[r][t] = z;
             }
         }
-        if (kAhead && b + kKaWaves < j.b1) load_k(b + kKaWaves);
+        if (kAhead && b + NW < j.b1) load_k(b + NW);
         if (kLateV) load_v(b);
         if (lim < kKvBlock || (!pre && first_own - key0 < kKvBlock)) {
 #pragma unroll
@@ -430,7 +454,7 @@ __device__ __forceinline__ void ka_stream(const KaArgs& a, const KaJob& j, KaStr
                 for (int i = 0; i < 4; ++i) o[r][d][i] = __builtin_fmaf(o[r][d][i], beta[r], z[i]);
             }
         }
-        if (kAhead && b + kKaWaves < j.b1) load_v(b + kKaWaves);
+        if (kAhead && b + NW < j.b1) load_v(b + NW);
     }
     // join the waves' sums
 #pragma unroll
@@ -446,7 +470,7 @@ __device__ __forceinline__ void ka_stream(const KaArgs& a, const KaJob& j, KaStr
     for (int r = 0; r < RT; ++r) {
         float mm = sh.ml[0][r * 16 + c].x;
 #pragma unroll
-        for (int w = 1; w < kKaWaves; ++w) mm = fmaxf(mm, sh.ml[w][r * 16 + c].x);
+        for (int w = 1; w < NW; ++w) mm = fmaxf(mm, sh.ml[w][r * 16 + c].x);
         const float e = st[r].l == 0.f ? 0.f : __builtin_amdgcn_exp2f(st[r].m - mm) * sgn;
 #pragma unroll
         for (int d = 0; d < DT; ++d)
@@ -455,20 +479,20 @@ __device__ __forceinline__ void ka_stream(const KaArgs& a, const KaJob& j, KaStr
                 sh.o[wave][r * 16 + c][d * 16 + g * 4 + i] = st[r].l == 0.f ? 0.f : o[r][d][i] * e;
     }
     __syncthreads();
-    for (int it = tid; it < M * (HD / 4); it += 64 * kKaWaves) {
+    for (int it = tid; it < M * (HD / 4); it += 64 * NW) {
         const int rr = it / (HD / 4), d = it % (HD / 4) * 4, row = j.r0 + rr;
         if (row >= j.r1) continue;
         float mm = sh.ml[0][rr].x, l = 0.f;
 #pragma unroll
-        for (int w = 1; w < kKaWaves; ++w) mm = fmaxf(mm, sh.ml[w][rr].x);
+        for (int w = 1; w < NW; ++w) mm = fmaxf(mm, sh.ml[w][rr].x);
         kq_f4 v = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int w = 0; w < kKaWaves; ++w) {
+        for (int w = 0; w < NW; ++w) {
             const float2 ml = sh.ml[w][rr];
             if (ml.y != 0.f) l += ml.y * __builtin_amdgcn_exp2f(ml.x - mm);
             v += *(const kq_f4*)&sh.o[w][rr][d];
         }
-        const int tok = row / a.group, head = j.kv * a.group + (row - tok * a.group);
+        const int tok = a.by_group(row), head = j.kv * a.group + (row - tok * a.group);
         if (direct) {
             const bool live = j.start >= 0 && j.start + (int64_t)(tok - j.seq * a.n_tok) < a.limit;
             const float inv = (TY == ORC_F16 ? 1.f : 0.0625f) / l;
@@ -557,22 +581,33 @@ template <int TY, int HD> struct KaStage {
     }
 };
 
-template <int HD> struct KaTileLds {
-    uint8_t t[2][2][kKvBlock * HD * 2];  // [buffer][K, V]
+template <int HD, int RT, int KG> union KaTileLds {
+    uint8_t t[KG][2][2][kKvBlock * HD * 2];  // [key group][buffer][K, V]
+    struct {                                 // the second key group's sums
+        float o[HD / 16][4 * RT * 64 * 4];   // [dim tile][wave, row tile, lane, dim]
+        float2 ml[4 * RT * 64];
+    } join;
 };
 
-template <int TY, int HD, int RT>
-__device__ __forceinline__ void ka_tile(const KaArgs& a, const KaJob& j, KaTileLds<HD>& sh) {
+template <int TY, int HD, int RT, int KG>
+__device__ __forceinline__ void ka_tile(const KaArgs& a, KaJob j, KaTileLds<HD, RT, KG>& sh) {
     constexpr int DT = HD / 16, KS = HD / 32, BB = kvq_block_bytes(TY, HD);
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 15, g = lane >> 4;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6) & 3, kg = KG == 1 ? 0 : __builtin_amdgcn_readfirstlane(tid >> 8), c = lane & 15, g = lane >> 4;
+    const int w0 = j.r0 + wave * 16 * RT;  // the wave's first row
+    KaRaw<HD> raw[RT];  // asked for before the position that the keys depend on is there
+#pragma unroll
+    for (int r = 0; r < RT; ++r) {
+        const int row = min(w0 + r * 16 + c, j.r1 - 1), tok = a.by_group(row), hg = row - tok * a.group;
+        raw[r].load(a.q + (int64_t)tok * a.ldq + (size_t)(j.kv * a.group + hg) * HD, g);
+    }
+    ka_keys(a, j);
     const bool direct = a.cp + a.co == 1;
     if (j.b0 >= j.b1 && !direct) return;
     const int nbp = (a.prefix + kKvBlock - 1) / kKvBlock;
-    const int w0 = j.r0 + wave * 16 * RT;  // the wave's first row
 
     // own rows that the wave's first and last row see
-    const int first_own = j.seq < 0 ? 0 : min(j.start + w0 / a.group - j.seq * a.n_tok + 1, j.len);
-    const int last_own = j.seq < 0 ? 0 : min(j.start + (min(w0 + 16 * RT, j.r1) - 1) / a.group - j.seq * a.n_tok + 1, j.len);
+    const int first_own = j.seq < 0 ? 0 : min(j.start + a.by_group(w0) - j.seq * a.n_tok + 1, j.len);
+    const int last_own = j.seq < 0 ? 0 : min(j.start + a.by_group(min(w0 + 16 * RT, j.r1) - 1) - j.seq * a.n_tok + 1, j.len);
     const bool rows = w0 < j.r1;
     const uint8_t* pk = a.pk + (size_t)j.kv * (a.pctx / kKvBlock) * BB;
     const uint8_t* pv = a.pv + (size_t)j.kv * (a.pctx / kKvBlock) * BB;
@@ -586,34 +621,34 @@ __device__ __forceinline__ void ka_tile(const KaArgs& a, const KaJob& j, KaTileL
     auto limit = [&](int b) { return b < nbp ? a.prefix - b * kKvBlock : j.len - (b - nbp) * kKvBlock; };
     auto put = [&](int b, int buf) {
         if (limit(b) < kKvBlock) sg.keep(limit(b), lane);
-        sg.put(sh.t[buf][0], sh.t[buf][1], wave, lane, buf ? 0u : 0x80008000u);
+        sg.put(sh.t[kg][buf][0], sh.t[kg][buf][1], wave, lane, buf ? 0u : 0x80008000u);
     };
     const float minus = ka_minus();
     float sgn = 1.f;
-    if (j.b0 < j.b1) load(j.b0);  // on its way while q is split
+    const int bg = j.b0 + kg;  // the key group's first block; it takes every KG-th
+    if (bg < j.b1) load(bg);  // on its way while q is split
     KaQ<TY, HD> q[RT];
     KaRow st[RT];
     int vis[RT];
     kq_f4 o[RT][DT];
 #pragma unroll
     for (int r = 0; r < RT; ++r) {
-        const int row = w0 + r * 16 + c, tok = row / a.group, hg = row - tok * a.group;
-        q[r].load(a.q + (int64_t)tok * a.ldq + (size_t)(j.kv * a.group + hg) * HD, row < j.r1, g);
+        const int tok = a.by_group(min(w0 + r * 16 + c, j.r1 - 1));
+        q[r].split(raw[r]);
         vis[r] = j.seq < 0 ? 0 : min(j.start + tok - j.seq * a.n_tok + 1, j.len);
 #pragma unroll
         for (int d = 0; d < DT; ++d) o[r][d] = kq_f4{0.f, 0.f, 0.f, 0.f};
     }
-    if (j.b0 < j.b1) {
-        put(j.b0, 0);
-        load(min(j.b0 + 1, j.b1 - 1));
+    if (bg < j.b1) {
+        put(bg, 0);
+        load(min(bg + KG, j.b1 - 1));
     }
     __syncthreads();
-    for (int b = j.b0; b < j.b1; ++b) {
-        const int cur = (b - j.b0) & 1;
+    for (int b = bg, cur = 0; b < j.b1 + kg; b += KG, cur ^= 1) {  // every group as many rounds as the first
         const bool pre = b < nbp;
         const int key0 = (pre ? b : b - nbp) * kKvBlock, lim = limit(b);
-        const uint8_t *kt = sh.t[cur][0] + lane * 16, *vt = sh.t[cur][1] + lane * 16;
-        if (rows && (pre || key0 < last_own)) {
+        const uint8_t *kt = sh.t[kg][cur][0] + lane * 16, *vt = sh.t[kg][cur][1] + lane * 16;
+        if (rows && b < j.b1 && (pre || key0 < last_own)) {
             sgn = cur ? 1.f : -1.f;
             kq_f4 s[RT][4];
 #pragma unroll
@@ -666,11 +701,33 @@ __device__ __forceinline__ void ka_tile(const KaArgs& a, const KaJob& j, KaTileL
             }
         }
         // the next block into the other buffer (read last before the barrier that ended the block before this one)
-        if (b + 1 < j.b1) {
-            put(b + 1, cur ^ 1);
-            load(min(b + 2, j.b1 - 1));
+        if (b + KG < j.b1) {
+            put(b + KG, cur ^ 1);
+            load(min(b + 2 * KG, j.b1 - 1));
         }
         __syncthreads();
+    }
+    if constexpr (KG == 2) {
+#pragma unroll
+        for (int r = 0; r < RT; ++r)
+            if (kg) {
+                sh.join.ml[(wave * RT + r) * 64 + lane] = make_float2(st[r].m, st[r].l);
+#pragma unroll
+                for (int d = 0; d < DT; ++d) *(kq_f4*)&sh.join.o[d][((wave * RT + r) * 64 + lane) * 4] = o[r][d] * sgn;
+            }
+        __syncthreads();
+        if (kg) return;
+#pragma unroll
+        for (int r = 0; r < RT; ++r) {
+            const float2 ml = sh.join.ml[(wave * RT + r) * 64 + lane];
+            const float mm = ka_max(st[r].m, ml.x), ref = mm == -__builtin_inff() ? 0.f : mm;
+            const float e0 = __builtin_amdgcn_exp2f(st[r].m - ref), e1 = __builtin_amdgcn_exp2f(ml.x - ref);
+            st[r].m = mm;
+            st[r].l = st[r].l * e0 + ml.y * e1;
+#pragma unroll
+            for (int d = 0; d < DT; ++d) o[r][d] = o[r][d] * (e0 * sgn) + *(const kq_f4*)&sh.join.o[d][((wave * RT + r) * 64 + lane) * 4] * e1;
+        }
+        sgn = 1.f;
     }
 #pragma unroll
     for (int r = 0; r < RT; ++r) {
@@ -679,7 +736,7 @@ __device__ __forceinline__ void ka_tile(const KaArgs& a, const KaJob& j, KaTileL
         l += __shfl_xor(l, 32, 64);
         const int row = w0 + r * 16 + c;
         if (row >= j.r1) continue;
-        const int tok = row / a.group, head = j.kv * a.group + (row - tok * a.group);
+        const int tok = a.by_group(row), head = j.kv * a.group + (row - tok * a.group);
         if (direct) {
             const bool live = j.start >= 0 && j.start + (int64_t)(tok - j.seq * a.n_tok) < a.limit && l != 0.f;
             const float inv = sgn * (TY == ORC_F16 ? 1.f : 0.0625f) / l;
@@ -700,28 +757,28 @@ __device__ __forceinline__ void ka_tile(const KaArgs& a, const KaJob& j, KaTileL
 }
 
 // ── kernels ──────────────────────────────────────────────────────────────────
-template <int TY, int HD, int RT> __global__ __launch_bounds__(64 * kKaWaves) void k_attn_kvq(KaArgs a) {
-    __shared__ __attribute__((aligned(16))) KaStreamLds<HD, RT> sh;
+template <int TY, int HD, int RT> __global__ __launch_bounds__(256) void k_attn_kvq(KaArgs a) {
+    __shared__ __attribute__((aligned(16))) KaStreamLds<HD, RT, 4> sh;
     KaJob j;
-    if (ka_job(a, 16 * RT, 16 * RT, j)) ka_stream<TY, HD, RT>(a, j, sh);
+    if (ka_rows(a, 16 * RT, 16 * RT, j)) ka_stream<TY, HD, RT, 4>(a, j, sh);
 }
 
-template <int TY, int HD, int RT> __global__ __launch_bounds__(64 * kKaWaves, 2) void k_attn_kvq_tile(KaArgs a) {
-    __shared__ __attribute__((aligned(16))) KaTileLds<HD> sh;
+template <int TY, int HD, int RT, int KG> __global__ __launch_bounds__(256 * KG, 2) void k_attn_kvq_tile(KaArgs a) {
+    __shared__ __attribute__((aligned(16))) KaTileLds<HD, RT, KG> sh;
     KaJob j;
-    if (ka_job(a, 64 * RT, 64 * RT, j)) ka_tile<TY, HD, RT>(a, j, sh);
+    if (ka_rows(a, 64 * RT, 64 * RT, j)) ka_tile<TY, HD, RT, KG>(a, j, sh);
 }
 
 // Prefix jobs of many rows and own jobs of few in one launch: the own ones fill the CUs that the prefix leaves idle.
-template <int TY, int HD, int RP, int RO> __global__ __launch_bounds__(64 * kKaWaves, 2) void k_attn_kvq_both(KaArgs a) {
+template <int TY, int HD, int RP, int RO> __global__ __launch_bounds__(256, 2) void k_attn_kvq_both(KaArgs a) {
     __shared__ __attribute__((aligned(16))) union {
-        KaTileLds<HD> t;
-        KaStreamLds<HD, RO> s;
+        KaTileLds<HD, RP, 1> t;
+        KaStreamLds<HD, RO, 4> s;
     } sh;
     KaJob j;
-    if (!ka_job(a, 64 * RP, 16 * RO, j)) return;
-    if (j.seq < 0) ka_tile<TY, HD, RP>(a, j, sh.t);
-    else ka_stream<TY, HD, RO>(a, j, sh.s);
+    if (!ka_rows(a, 64 * RP, 16 * RO, j)) return;
+    if (j.seq < 0) ka_tile<TY, HD, RP, 1>(a, j, sh.t);
+    else ka_stream<TY, HD, RO, 4>(a, j, sh.s);
 }
 
 // ── the chunks' partial sums ─────────────────────────────────────────────────
@@ -736,8 +793,25 @@ template <int HD, int W> __global__ __launch_bounds__(256) void k_attn_kvq_merge
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, sub = wave / W;
     const int64_t row = (int64_t)blockIdx.x * R + sub;
     const bool some = row < a.n_rows;
-    const int tok = some ? (int)(row / a.n_heads) : 0, head = some ? (int)(row - (int64_t)tok * a.n_heads) : 0, seq = tok / a.n_tok;
-    const int start = kvq_start(a.d_pos, seq, a.pos_off, a.limit), n = a.cp + a.co;
+    const int tok = some ? a.by_heads((int)row) : 0, head = some ? (int)row - tok * a.n_heads : 0, seq = a.by_tok(tok);
+    const int n = a.cp + a.co;
+    // the first chunks' sums and rows are asked for before the position is there; what an unwritten chunk holds is dropped
+    const float* po = a.part_o + (size_t)(some ? row : 0) * HD + lane * E;
+    const float2* pm = a.part_ml + (some ? row : 0);
+    const size_t step = (size_t)a.n_rows * HD;
+    float2 ml[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) ml[u] = pm[(size_t)min(lane + u * 64, n - 1) * a.n_rows];
+    constexpr int U = 8;
+    float x[U][E];
+    auto ask = [&](int c0) {
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int i = 0; i < E; ++i) x[u][i] = po[(size_t)min(c0 + u * W, n - 1) * step + i];
+    };
+    ask(wave % W);
+    const int start = kvq_start(a.d_pos, seq, a.pos_off, a.limit);
     const bool live = some && start >= 0 && start + (int64_t)(tok - seq * a.n_tok) < a.limit;
     float v[E] = {};
     float l = 0.f;
@@ -749,20 +823,18 @@ template <int HD, int W> __global__ __launch_bounds__(256) void k_attn_kvq_merge
         float m = -__builtin_inff();
         auto get = [&](int c) {  // (maximum, sum) of chunk c; (-inf, 0) where it holds nothing of the row
             int b0, b1;
-            if (c < a.cp) ka_chunk(nbp, a.cp, c, b0, b1);
-            else ka_chunk(nb, a.co, c - a.cp, b0, b1);
+            if (c < a.cp) ka_chunk(nbp, a.by_cp, c, b0, b1);
+            else ka_chunk(nb, a.by_co, c - a.cp, b0, b1);
             if (c >= n || b0 >= b1 || (c >= a.cp && b0 > last)) return make_float2(-__builtin_inff(), 0.f);
-            return a.part_ml[(size_t)c * a.n_rows + row];
+            return c < 64 ? ml[0] : c < 128 ? ml[1] : pm[(size_t)c * a.n_rows];
         };
-        const float2 mine = get(lane);
-        m = mine.x;
-        for (int c = lane + 64; c < n; c += 64) m = fmaxf(m, get(c).x);
+        for (int c = lane; c < n; c += 64) m = fmaxf(m, get(c).x);
 #pragma unroll
         for (int d = 32; d; d >>= 1) m = fmaxf(m, __shfl_xor(m, d, 64));
         for (int c = lane; c < n; c += 64) {
-            const float2 ml = c == lane ? mine : get(c);
-            const float e = ml.y == 0.f ? 0.f : __builtin_amdgcn_exp2f(ml.x - m);
-            if (ml.y != 0.f) l += e * ml.y;
+            const float2 y = get(c);
+            const float e = y.y == 0.f ? 0.f : __builtin_amdgcn_exp2f(y.x - m);
+            if (y.y != 0.f) l += e * y.y;
             if (W == 1 || wave == 0) wt[sub][c] = e;
         }
 #pragma unroll
@@ -770,21 +842,14 @@ template <int HD, int W> __global__ __launch_bounds__(256) void k_attn_kvq_merge
     }
     __syncthreads();
     if (live) {
-        const float* po = a.part_o + (size_t)row * HD + lane * E;
-        const size_t step = (size_t)a.n_rows * HD;
-        for (int c0 = wave % W; c0 < n; c0 += W * 8) {  // eight loads at a time; what an unwritten chunk holds is dropped
-            float x[8][E], e[8];
+        for (int c0 = wave % W; c0 < n; c0 += W * U) {
+            if (c0 >= W) ask(c0);
 #pragma unroll
-            for (int u = 0; u < 8; ++u) {
-                const int c = c0 + u * W;
-                e[u] = c < n ? wt[sub][c] : 0.f;
+            for (int u = 0; u < U; ++u) {
+                const float e = c0 + u * W < n ? wt[sub][c0 + u * W] : 0.f;
 #pragma unroll
-                for (int i = 0; i < E; ++i) x[u][i] = po[(size_t)min(c, n - 1) * step + i];
+                for (int i = 0; i < E; ++i) v[i] += e == 0.f ? 0.f : e * x[u][i];
             }
-#pragma unroll
-            for (int u = 0; u < 8; ++u)
-#pragma unroll
-                for (int i = 0; i < E; ++i) v[i] += e[u] == 0.f ? 0.f : e[u] * x[u][i];
         }
     }
     if constexpr (W > 1) {
@@ -804,23 +869,28 @@ template <int HD, int W> __global__ __launch_bounds__(256) void k_attn_kvq_merge
 }
 
 // ── host ─────────────────────────────────────────────────────────────────────
-constexpr int kKaFill = 512;  // workgroups that fill the card: two on each CU
-
 struct KaPlan {
     bool shared;
     int m_p, m_o;  // rows of a workgroup: 16 or 32 (the waves share out the keys), 64 or 128 (they share the operands)
+    int kg;        // key groups of the 64-row workgroups: 4 waves each
     int tiles_p, cp, tiles_o, co;
     size_t rows;
     int slots() const { return cp + co; }
     size_t bytes(int hd) const { return slots() > 1 ? (size_t)slots() * rows * (4 * (size_t)hd + 8) : 0; }
 };
 
+static KaDiv ka_fast(int d) {
+    KaDiv r{0, 0, std::max(d, 1)};
+    while (((int64_t)1 << r.shift) < r.d) ++r.shift;
+    if (r.d > 1) r.mul = (uint32_t)((((uint64_t)1 << (31 + r.shift)) / r.d) + 1);
+    return r;
+}
+
 static int ka_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 
 // Chunks of nb key blocks for `base` workgroups' worth of row tiles: at most `most` workgroups, and four blocks each or
 // more, all of a length but the last; one where `one` blocks are no more work than a second launch.
 static int ka_chunks(int64_t base, int nb, int64_t most, int one) {
-    if (getenv("KA_ONE")) one = atoi(getenv("KA_ONE"));
     if (nb <= one) return 1;
     const int n = (int)std::max<int64_t>(1, std::min<int64_t>(most / base, (nb + 3) / 4));
     return ka_div(nb, ka_div(nb, n));
@@ -833,31 +903,36 @@ static KaPlan ka_plan(int n_seq, int n_tok, int n_heads, int n_kv, int prefix_le
     const int nbp = ka_div(prefix_len, kKvBlock), nbo = ka_div(pos_limit, kKvBlock);
     // with this many rows each, sequences gain nothing from common tiles
     p.shared = prefix_len > 0 && n_seq > 1 && rows_o < 128;
+    p.kg = 1;
     if (p.shared) {
         p.m_p = rows_p <= 16 ? 16 : rows_p <= 32 ? 32 : n_kv * (int64_t)ka_div(rows_p, 128) * (nbp / 8) >= 512 ? 128 : 64;
         p.m_o = p.m_p <= 32 ? p.m_p : rows_o <= 16 ? 16 : rows_o <= 32 ? 32 : p.m_p;
-    } else
+    } else {
         p.m_o = rows_o <= 16 ? 16 : rows_o <= 32 ? 32 : (int64_t)n_seq * n_kv * ka_div(rows_o, 128) >= 1024 ? 128 : 64;
+        if (p.m_o == 64 && (int64_t)n_seq * n_kv * ka_div(rows_o, 64) * ka_div(nbp + nbo, 4) < 2048) p.kg = 2;
+    }
     p.tiles_o = ka_div(rows_o, p.m_o);
-    const int64_t base_o = (int64_t)n_seq * n_kv * p.tiles_o;
-    p.co = ka_chunks(base_o, p.shared ? nbo : nbp + nbo, kKaFill, p.m_o <= 32 ? 12 : 4);
+    const int64_t base_o = (int64_t)n_seq * n_kv * p.tiles_o, fill = 512 / p.kg;  // workgroups that fill the card
+    p.co = ka_chunks(base_o, p.shared ? nbo : nbp + nbo, fill, p.m_o <= 32 ? 12 : 4 * p.kg);
     if (p.shared) {
         p.tiles_p = ka_div(rows_p, p.m_p);
         const int64_t base_p = (int64_t)n_kv * p.tiles_p;
         // short prefix chunks share the card with the own jobs; beside long ones those are done in passing
-        const bool lng = nbp * base_p >= 16 * kKaFill;
-        p.cp = ka_chunks(base_p, nbp, lng ? kKaFill : std::max<int64_t>(kKaFill / 2, kKaFill - base_o * p.co), 4);
+        const bool lng = nbp * base_p >= 16 * fill;
+        p.cp = ka_chunks(base_p, nbp, lng ? fill : std::max<int64_t>(fill / 2, fill - base_o * p.co), 4);
     }
     return p;
 }
 
 template <int TY, int HD> static void ka_launch(const KaPlan& p, const KaArgs& a, hipStream_t s) {
-    auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(8 * ((unsigned)(a.jobs_p + 7) / 8 + (unsigned)(a.jobs_o + 7) / 8)), dim3(64 * kKaWaves), 0, s, a); };
+    auto go = [&](auto kernel) {
+        hipLaunchKernelGGL(kernel, dim3(8 * ((unsigned)(a.jobs_p + 7) / 8 + (unsigned)(a.jobs_o + 7) / 8)), dim3(256 * p.kg), 0, s, a);
+    };
     if (!p.shared || p.m_p == p.m_o) {
         if (p.m_o == 16) go(k_attn_kvq<TY, HD, 1>);
         else if (p.m_o == 32) go(k_attn_kvq<TY, HD, 2>);
-        else if (p.m_o == 64) go(k_attn_kvq_tile<TY, HD, 1>);
-        else go(k_attn_kvq_tile<TY, HD, 2>);
+        else if (p.m_o == 64) p.kg == 1 ? go(k_attn_kvq_tile<TY, HD, 1, 1>) : go(k_attn_kvq_tile<TY, HD, 1, 2>);
+        else go(k_attn_kvq_tile<TY, HD, 2, 1>);
     } else if (p.m_p == 64) p.m_o == 16 ? go(k_attn_kvq_both<TY, HD, 1, 1>) : go(k_attn_kvq_both<TY, HD, 1, 2>);
     else p.m_o == 16 ? go(k_attn_kvq_both<TY, HD, 2, 1>) : go(k_attn_kvq_both<TY, HD, 2, 2>);
 }
@@ -903,7 +978,9 @@ extern "C" int orc_attn_kvq(int type, const float* d_q, int ldq, int n_seq, int 
     if (jobs_p + jobs_o > 0xffffff00ll / 256 - 16) return set_error(ORC_E_INVALID, "attn_kvq: too many rows");
     KaArgs a{d_q, ldq, n_seq, n_tok, n_heads, n_kv, n_heads / n_kv, (const uint8_t*)d_pk, (const uint8_t*)d_pv,
              (const uint8_t*)d_kc, (const uint8_t*)d_vc, prefix_len, prefix_ctx, ctx, d_pos, pos_off, pos_limit, d_out,
-             ldo, nullptr, nullptr, (int)p.rows, p.shared, p.tiles_p, p.cp, p.tiles_o, p.co, (int)jobs_p, (int)jobs_o};
+             ldo, nullptr, nullptr, (int)p.rows, p.shared, p.tiles_p, p.cp, p.tiles_o, p.co, (int)jobs_p, (int)jobs_o,
+             ka_fast(n_heads / n_kv), ka_fast(n_kv), ka_fast(p.tiles_p), ka_fast(p.cp), ka_fast(p.tiles_o), ka_fast(p.co),
+             ka_fast(n_heads), ka_fast(n_tok)};
     if (bytes) {
         a.part_o = (float*)d_work;
         a.part_ml = (float2*)((uint8_t*)d_work + (size_t)p.slots() * p.rows * head_dim * 4);
