@@ -79,7 +79,12 @@ __device__ __forceinline__ bool ka_rows(const KaArgs& a, int m_p, int m_o, KaJob
         j.r1 = min(j.r0 + m_p, a.n_seq * a.n_tok * a.group);
         return true;
     }
-    const int t = a.by_tiles_o(w), tile = (t + 1) * a.tiles_o - 1 - w;  // the longest rows first
+    // The longest rows first, every other 32 of them the other way round: an XCD's 32 CUs take workgroups in turn, and
+    // so each gets long and short ones.
+    const int t = a.by_tiles_o(w);
+    int tile = w - t * a.tiles_o;
+    if ((tile & 32) && (tile | 31) < a.tiles_o) tile ^= 31;
+    tile = a.tiles_o - 1 - tile;
     const int sk = a.by_co(t), rows = a.n_tok * a.group;
     j.slot = a.cp + t - sk * a.co;
     j.seq = a.by_kv(sk);
