@@ -269,8 +269,7 @@ template <int HD> struct KaRaw {
 };
 template <int TY, int HD> struct KaQ {
     kq_h8 hi[HD / 32], lo[HD / 32];
-    float f;
-    __device__ __forceinline__ void split(const KaRaw<HD>& x) {
+    __device__ __forceinline__ void split(const KaRaw<HD>& x, float& f) {
         float mx = 0.f;
 #pragma unroll
         for (int i = 0; i < HD / 16; ++i)
@@ -298,14 +297,11 @@ __device__ __forceinline__ kq_f4 ka_mfma(kq_h8 a, kq_h8 b, kq_f4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }
 
-// Running softmax of one row (per lane; the four lanes of a row agree on m,
-// each sums its own keys).
+// Running softmax of a row (per lane; the four lanes of a row agree on m and c, each sums its own keys).
 struct KaRow {
     float m = -__builtin_inff(), l = 0.f;
-    // scores s of the lane's 16 keys -> weights times 2^15 (SIGN: and the sign bit); returns what the sums so far are
-    // scaled by
-    template <bool SIGN>
-    __device__ __forceinline__ float step(kq_f4 (&s)[4], float f, float minus, uint32_t sign, u32x4 (&hi)[2], u32x4 (&lo)[2]) {
+    float c = 15.f;  // 15 less the reference that the weights are formed against
+    __device__ __forceinline__ float largest(const kq_f4 (&s)[4]) const {
         float mx = ka_max(ka_max(s[0][0], s[0][1]), s[0][2]);
         mx = ka_max(ka_max(mx, s[0][3]), s[1][0]);
         mx = ka_max(ka_max(mx, s[1][1]), s[1][2]);
@@ -313,19 +309,28 @@ struct KaRow {
         mx = ka_max(ka_max(mx, s[2][1]), s[2][2]);
         mx = ka_max(ka_max(mx, s[2][3]), s[3][0]);
         mx = ka_max(ka_max(mx, s[3][1]), s[3][2]);
-        mx = ka_max(mx, s[3][3]);
+        return ka_max(mx, s[3][3]);
+    }
+    // A new reference for the row whose lanes' largest score is mx; returns what the sums so far are scaled by.
+    __device__ __forceinline__ float raise(float mx) {
         mx = ka_max(ka_max(mx, __shfl_xor(mx, 16, 64)), __shfl_xor(mx, 32, 64));
         mx = ka_max(mx, __shfl_xor(mx, 48, 64));
-        const float mn = ka_max(m, mx * f), ref = mn == -__builtin_inff() ? 0.f : mn;
-        const float alpha = __builtin_amdgcn_exp2f(m - ref);
+        const float mn = ka_max(m, mx), ref = mn == -__builtin_inff() ? 0.f : mn, alpha = __builtin_amdgcn_exp2f(m - ref);
         m = mn;
+        c = 15.f - ref;
+        l *= alpha;
+        return alpha;
+    }
+    // Scores -> weights times 2^15, in two halves (SIGN: and the sign bit)
+    template <bool SIGN>
+    __device__ __forceinline__ void weigh(const kq_f4 (&s)[4], float f, float minus, uint32_t sign, u32x4 (&hi)[2], u32x4 (&lo)[2]) {
         float sum = 0.f;
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
             float p[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                p[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][i], f, 15.f - ref));
+                p[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][i], f, c));
                 sum += p[i];
             }
             uint32_t l0, l1, h0 = ka_split(p[0], p[1], minus, l0), h1 = ka_split(p[2], p[3], minus, l1);
@@ -335,9 +340,56 @@ struct KaRow {
             lo[t / 2][(t & 1) * 2] = l0;
             lo[t / 2][(t & 1) * 2 + 1] = l1;
         }
-        l = l * alpha + sum;
-        return alpha;
+        l += sum;
     }
+};
+
+// The weights of a block's 64 keys (16 a lane) for RT row tiles; beta: less what the sums so far are scaled by. The
+// reference is a maximum seen before; it is raised, for all of the wave's rows, only when some score passes its row's
+// by so much (7/8) that a weight could pass fp16's range: after the first blocks hardly ever, and neither the exchanges
+// between lanes nor the scaling's exponential are on the way from the scores to the weights.
+template <bool SIGN, int RT>
+__device__ __forceinline__ void ka_weights(const kq_f4 (&s)[RT][4], const float (&f)[RT], float minus, uint32_t sign,
+                                           KaRow (&st)[RT], u32x4 (&hi)[RT][2], u32x4 (&lo)[RT][2], float (&beta)[RT]) {
+    float mx[RT];
+    bool over = false;
+#pragma unroll
+    for (int r = 0; r < RT; ++r) {
+        mx[r] = st[r].largest(s[r]) * f[r];
+        over |= !(mx[r] <= st[r].m + 0.875f);
+        beta[r] = -1.f;
+    }
+    // (two row tiles: always, which costs less there than two stretches of code that cannot be interleaved)
+    if (RT > 1 || __ballot(over)) {
+#pragma unroll
+        for (int r = 0; r < RT; ++r) beta[r] = -st[r].raise(mx[r]);
+    }
+#pragma unroll
+    for (int r = 0; r < RT; ++r) st[r].template weigh<SIGN>(s[r], f[r], minus, sign, hi[r], lo[r]);
+}
+
+// A job's key blocks by one number, the prefix's and then the own ones, so that block b's keys start at 64 b and the
+// own ones at 64 nbp: where their bytes are, how many of them there are, how many own ones a token sees.
+template <int BB> struct KaKeys {
+    const uint8_t *pk, *pv, *ok, *ov;
+    int nbp, end_p, end_o, first;
+    __device__ __forceinline__ KaKeys(const KaArgs& a, const KaJob& j) {
+        nbp = (a.prefix + kKvBlock - 1) / kKvBlock;
+        const size_t pre = (size_t)j.kv * (a.pctx / kKvBlock) * BB;
+        // (from block nbp on)
+        const size_t own = (((size_t)max(j.seq, 0) * a.n_kv + j.kv) * (a.ctx / kKvBlock) - nbp) * BB;
+        pk = a.pk + pre;
+        pv = a.pv + pre;
+        ok = a.kc + own;
+        ov = a.vc + own;
+        end_p = a.prefix;
+        end_o = nbp * kKvBlock + j.len;
+        first = nbp * kKvBlock + (j.seq < 0 ? 0 : j.start + 1 - j.seq * a.n_tok);
+    }
+    __device__ __forceinline__ const uint8_t* k(int b) const { return (b < nbp ? pk : ok) + (size_t)b * BB; }
+    __device__ __forceinline__ const uint8_t* v(int b) const { return (b < nbp ? pv : ov) + (size_t)b * BB; }
+    __device__ __forceinline__ int limit(int b) const { return (b < nbp ? end_p : end_o) - b * kKvBlock; }  // keys from b's first
+    __device__ __forceinline__ int sees(int tok) const { return min(first + tok, end_o); }  // end of the keys a token sees
 };
 
 // ── few rows: the waves share out the keys ───────────────────────────────────
@@ -361,22 +413,18 @@ __device__ __forceinline__ void ka_stream(const KaArgs& a, KaJob j, KaStreamLds<
     ka_keys(a, j);
     const bool direct = a.cp + a.co == 1;
     if (j.b0 >= j.b1 && !direct) return;
-    const int nbp = (a.prefix + kKvBlock - 1) / kKvBlock;
-
-    const int first_own = j.seq < 0 ? 0 : min(j.start + a.by_group(j.r0) - j.seq * a.n_tok + 1, j.len);  // the least vis
-    const uint8_t* pk = a.pk + (size_t)j.kv * (a.pctx / kKvBlock) * BB;
-    const uint8_t* pv = a.pv + (size_t)j.kv * (a.pctx / kKvBlock) * BB;
-    const size_t own = ((size_t)max(j.seq, 0) * a.n_kv + j.kv) * (a.ctx / kKvBlock) * BB;
+    const KaKeys<BB> keys(a, j);
+    const int least = keys.sees(a.by_group(j.r0));  // what the first row sees
     KaK<TY, HD> kr[4] = {};
     KaV<TY, HD> vr = {};
     uint32_t ks = 0;
     auto load_k = [&](int b) {
-        const uint8_t* kb = b < nbp ? pk + (size_t)b * BB : a.kc + own + (size_t)(b - nbp) * BB;
+        const uint8_t* kb = keys.k(b);
 #pragma unroll
         for (int t = 0; t < 4; ++t) kr[t].load(kb, t, lane);
         if constexpr (TY != ORC_F16) ks = *(const uint32_t*)(kb + kvq_code_bytes(TY, HD) + ((HD == 128 ? g : g >> 1) * 16 + c) * 4);
     };
-    auto load_v = [&](int b) { vr.load(b < nbp ? pv + (size_t)b * BB : a.vc + own + (size_t)(b - nbp) * BB, lane); };
+    auto load_v = [&](int b) { vr.load(keys.v(b), lane); };
     // One row tile: a block's bytes are on their way while q is split and while the block before it is worked on. Two
     // row tiles, or 128 fp16 dims (128 registers of bytes), leave no registers for that, and both together none for V
     // before K is done with.
@@ -386,26 +434,27 @@ __device__ __forceinline__ void ka_stream(const KaArgs& a, KaJob j, KaStreamLds<
         load_v(j.b0 + wave);
     }
     KaQ<TY, HD> q[RT];
+    float f[RT];
     KaRow st[RT];
-    int vis[RT];  // own rows that the lane's query row sees
+    int vis[RT];  // end of the keys that the lane's query row sees
     kq_f4 o[RT][DT];
 #pragma unroll
     for (int r = 0; r < RT; ++r) {
         const int tok = a.by_group(min(j.r0 + r * 16 + c, j.r1 - 1));
-        q[r].split(raw[r]);
-        vis[r] = j.seq < 0 ? 0 : min(j.start + tok - j.seq * a.n_tok + 1, j.len);
+        q[r].split(raw[r], f[r]);
+        vis[r] = keys.sees(tok);
 #pragma unroll
         for (int d = 0; d < DT; ++d) o[r][d] = kq_f4{0.f, 0.f, 0.f, 0.f};
     }
     const float minus = ka_minus();
     float sgn = 1.f;
     for (int b = j.b0 + wave; b < j.b1; b += NW) {
-        const bool pre = b < nbp;
+        const bool pre = b < keys.nbp;
         if (!kAhead) {
             load_k(b);
             if (!kLateV) load_v(b);
         }
-        const int key0 = (pre ? b : b - nbp) * kKvBlock, lim = (pre ? a.prefix : j.len) - key0;
+        const int key0 = b * kKvBlock, lim = keys.limit(b);
         kq_f4 s[RT][4];
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
@@ -426,7 +475,7 @@ __device__ __forceinline__ void ka_stream(const KaArgs& a, KaJob j, KaStreamLds<
         }
         if (kAhead && b + NW < j.b1) load_k(b + NW);
         if (kLateV) load_v(b);
-        if (lim < kKvBlock || (!pre && first_own - key0 < kKvBlock)) {
+        if (lim < kKvBlock || (!pre && least - key0 < kKvBlock)) {
 #pragma unroll
             for (int r = 0; r < RT; ++r) {
                 const int n = pre ? lim : min(lim, vis[r] - key0);
@@ -443,8 +492,7 @@ __device__ __forceinline__ void ka_stream(const KaArgs& a, KaJob j, KaStreamLds<
         const uint32_t sign = sgn < 0.f ? 0x80008000u : 0u;
         u32x4 ph[RT][2], pl[RT][2];
         float beta[RT];
-#pragma unroll
-        for (int r = 0; r < RT; ++r) beta[r] = -st[r].template step<true>(s[r], q[r].f, minus, sign, ph[r], pl[r]);
+        ka_weights<true>(s, f, minus, sign, st, ph, pl, beta);
 #pragma unroll
         for (int d = 0; d < DT; ++d) {
             const kq_h8 v0 = vr.op(d, 0), v1 = vr.op(d, 1);
@@ -608,24 +656,15 @@ __device__ __forceinline__ void ka_tile(const KaArgs& a, KaJob j, KaTileLds<HD, 
     ka_keys(a, j);
     const bool direct = a.cp + a.co == 1;
     if (j.b0 >= j.b1 && !direct) return;
-    const int nbp = (a.prefix + kKvBlock - 1) / kKvBlock;
-
-    // own rows that the wave's first and last row see
-    const int first_own = j.seq < 0 ? 0 : min(j.start + a.by_group(w0) - j.seq * a.n_tok + 1, j.len);
-    const int last_own = j.seq < 0 ? 0 : min(j.start + a.by_group(min(w0 + 16 * RT, j.r1) - 1) - j.seq * a.n_tok + 1, j.len);
+    const KaKeys<BB> keys(a, j);
+    // ends of the keys that the wave's first and last row see
+    const int least = keys.sees(a.by_group(w0)), most = keys.sees(a.by_group(min(w0 + 16 * RT, j.r1) - 1));
     const bool rows = w0 < j.r1;
-    const uint8_t* pk = a.pk + (size_t)j.kv * (a.pctx / kKvBlock) * BB;
-    const uint8_t* pv = a.pv + (size_t)j.kv * (a.pctx / kKvBlock) * BB;
-    const size_t own = ((size_t)max(j.seq, 0) * a.n_kv + j.kv) * (a.ctx / kKvBlock) * BB;
     KaStage<TY, HD> sg = {};
-    auto load = [&](int b) {
-        const bool pre = b < nbp;
-        sg.load(pre ? pk + (size_t)b * BB : a.kc + own + (size_t)(b - nbp) * BB,
-                pre ? pv + (size_t)b * BB : a.vc + own + (size_t)(b - nbp) * BB, wave, lane);
-    };
-    auto limit = [&](int b) { return b < nbp ? a.prefix - b * kKvBlock : j.len - (b - nbp) * kKvBlock; };
+    auto load = [&](int b) { sg.load(keys.k(b), keys.v(b), wave, lane); };
     auto put = [&](int b, int buf) {
-        if (limit(b) < kKvBlock) sg.keep(limit(b), lane);
+        const int lim = keys.limit(b);
+        if (lim < kKvBlock) sg.keep(lim, lane);
         sg.put(sh.t[kg][buf][0], sh.t[kg][buf][1], wave, lane, buf ? 0u : 0x80008000u);
     };
     const float minus = ka_minus();
@@ -633,14 +672,15 @@ __device__ __forceinline__ void ka_tile(const KaArgs& a, KaJob j, KaTileLds<HD, 
     const int bg = j.b0 + kg;  // the key group's first block; it takes every KG-th
     if (bg < j.b1) load(bg);  // on its way while q is split
     KaQ<TY, HD> q[RT];
+    float f[RT];
     KaRow st[RT];
     int vis[RT];
     kq_f4 o[RT][DT];
 #pragma unroll
     for (int r = 0; r < RT; ++r) {
         const int tok = a.by_group(min(w0 + r * 16 + c, j.r1 - 1));
-        q[r].split(raw[r]);
-        vis[r] = j.seq < 0 ? 0 : min(j.start + tok - j.seq * a.n_tok + 1, j.len);
+        q[r].split(raw[r], f[r]);
+        vis[r] = keys.sees(tok);
 #pragma unroll
         for (int d = 0; d < DT; ++d) o[r][d] = kq_f4{0.f, 0.f, 0.f, 0.f};
     }
@@ -650,10 +690,10 @@ __device__ __forceinline__ void ka_tile(const KaArgs& a, KaJob j, KaTileLds<HD, 
     }
     __syncthreads();
     for (int b = bg, cur = 0; b < j.b1 + kg; b += KG, cur ^= 1) {  // every group as many rounds as the first
-        const bool pre = b < nbp;
-        const int key0 = (pre ? b : b - nbp) * kKvBlock, lim = limit(b);
+        const bool pre = b < keys.nbp;
+        const int key0 = b * kKvBlock, lim = keys.limit(b);
         const uint8_t *kt = sh.t[kg][cur][0] + lane * 16, *vt = sh.t[kg][cur][1] + lane * 16;
-        if (rows && b < j.b1 && (pre || key0 < last_own)) {
+        if (rows && b < j.b1 && (pre || key0 < most)) {
             sgn = cur ? 1.f : -1.f;
             kq_f4 s[RT][4];
 #pragma unroll
@@ -672,7 +712,7 @@ __device__ __forceinline__ void ka_tile(const KaArgs& a, KaJob j, KaTileLds<HD, 
 #pragma unroll
                     for (int r = 0; r < RT; ++r) s[r][t] = ka_mfma(k[i], q[r].hi[i], s[r][t]);
             }
-            if (lim < kKvBlock || (!pre && first_own - key0 < kKvBlock)) {
+            if (lim < kKvBlock || (!pre && least - key0 < kKvBlock)) {
 #pragma unroll
                 for (int r = 0; r < RT; ++r) {
                     const int n = pre ? lim : min(lim, vis[r] - key0);
@@ -685,8 +725,7 @@ __device__ __forceinline__ void ka_tile(const KaArgs& a, KaJob j, KaTileLds<HD, 
             }
             u32x4 ph[RT][2], pl[RT][2];
             float beta[RT];
-#pragma unroll
-            for (int r = 0; r < RT; ++r) beta[r] = -st[r].template step<false>(s[r], q[r].f, minus, 0u, ph[r], pl[r]);
+            ka_weights<false>(s, f, minus, 0u, st, ph, pl, beta);
 #pragma unroll
             for (int d = 0; d < DT; ++d) {
                 const kq_h8 v0 = *(const kq_h8*)(vt + d * 2048), v1 = *(const kq_h8*)(vt + d * 2048 + 1024);
@@ -901,7 +940,7 @@ static int ka_chunks(int64_t base, int nb, int64_t most, int one) {
     return ka_div(nb, ka_div(nb, n));
 }
 
-static KaPlan ka_plan(int n_seq, int n_tok, int n_heads, int n_kv, int prefix_len, int pos_limit) {
+static KaPlan ka_plan(int n_seq, int n_tok, int n_heads, int n_kv, int hd, int prefix_len, int pos_limit) {
     KaPlan p{};
     const int64_t group = n_heads / n_kv, rows_o = n_tok * group, rows_p = n_seq * rows_o;
     p.rows = (size_t)n_seq * n_tok * n_heads;
@@ -910,10 +949,15 @@ static KaPlan ka_plan(int n_seq, int n_tok, int n_heads, int n_kv, int prefix_le
     p.shared = prefix_len > 0 && n_seq > 1 && rows_o < 128;
     p.kg = 1;
     if (p.shared) {
-        p.m_p = rows_p <= 16 ? 16 : rows_p <= 32 ? 32 : n_kv * (int64_t)ka_div(rows_p, 128) * (nbp / 8) >= 512 ? 128 : 64;
+        p.m_p = rows_p <= 16 ? 16 : rows_p <= 32 ? 32 : n_kv * (int64_t)ka_div(rows_p, 128) * (nbp / 8) >= 384 ? 128 : 64;
         p.m_o = p.m_p <= 32 ? p.m_p : rows_o <= 16 ? 16 : rows_o <= 32 ? 32 : p.m_p;
     } else {
-        p.m_o = rows_o <= 16 ? 16 : rows_o <= 32 ? 32 : (int64_t)n_seq * n_kv * ka_div(rows_o, 128) >= 1024 ? 128 : 64;
+        // 128 rows share more work, 64 spread over more CUs: a prompt's first rows, which see few keys, want many
+        // workgroups to even out; rows behind a long context can have theirs by chunks of 8 blocks and more
+        const int64_t base = (int64_t)n_seq * n_kv * ka_div(rows_o, 128);
+        const bool many = 4 * (int64_t)n_tok > (int64_t)prefix_len + pos_limit ? base >= (hd == 64 ? 1024 : 640)
+                                                                               : base * ((nbp + nbo) / 8) >= 384;
+        p.m_o = rows_o <= 16 ? 16 : rows_o <= 32 ? 32 : many ? 128 : 64;
         if (p.m_o == 64 && (int64_t)n_seq * n_kv * ka_div(rows_o, 64) * ka_div(nbp + nbo, 4) < 2048) p.kg = 2;
     }
     p.tiles_o = ka_div(rows_o, p.m_o);
@@ -954,7 +998,7 @@ static bool ka_shape_ok(int n_seq, int n_tok, int n_heads, int n_kv, int prefix_
 extern "C" size_t orc_attn_kvq_workspace(int n_seq, int n_tok, int n_heads, int n_kv, int head_dim, int prefix_len,
                                          int pos_limit) {
     if ((head_dim != 64 && head_dim != 128) || !ka_shape_ok(n_seq, n_tok, n_heads, n_kv, prefix_len, pos_limit)) return 0;
-    return ka_plan(n_seq, n_tok, n_heads, n_kv, prefix_len, pos_limit).bytes(head_dim);
+    return ka_plan(n_seq, n_tok, n_heads, n_kv, head_dim, prefix_len, pos_limit).bytes(head_dim);
 }
 
 extern "C" int orc_attn_kvq(int type, const float* d_q, int ldq, int n_seq, int n_tok, int n_heads, int n_kv,
@@ -973,7 +1017,7 @@ extern "C" int orc_attn_kvq(int type, const float* d_q, int ldq, int n_seq, int 
                                         "prefix_len <= prefix_ctx, contexts multiples of 64)");
     if (!d_pos && (pos_off < 0 || (int64_t)pos_off + n_tok > pos_limit))
         return set_error(ORC_E_INVALID, "attn_kvq: positions must lie below pos_limit");
-    const KaPlan p = ka_plan(n_seq, n_tok, n_heads, n_kv, prefix_len, pos_limit);
+    const KaPlan p = ka_plan(n_seq, n_tok, n_heads, n_kv, head_dim, prefix_len, pos_limit);
     const size_t bytes = p.bytes(head_dim);
     if (!d_q || !d_out || !d_kc || !d_vc || (prefix_len && (!d_pk || !d_pv)) || (bytes && !d_work) ||
         (((uintptr_t)d_q | (uintptr_t)d_out | (uintptr_t)d_kc | (uintptr_t)d_vc | (uintptr_t)d_pk | (uintptr_t)d_pv |
