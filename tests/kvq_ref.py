@@ -67,22 +67,25 @@ def attention(q, pk, pv, k, v, starts, limit):
     """q [S][T][H][hd]; prefix pk, pv [KV][P][hd]; own k, v [S][KV][ctx][hd]. Returns (out, sum of w |v|, largest
     sum of |q k| / sqrt(hd) of each row, sum of |v|) in 64 bits."""
     S, T, H, hd = q.shape
-    KV = k.shape[1]
+    KV, P = k.shape[1], pk.shape[1]
+    G = H // KV
     out, scale, size, total = np.zeros(q.shape), np.zeros(q.shape), np.zeros(q.shape[:3] + (1,)), np.zeros(q.shape)
-    q = q.astype(np.float64)
-    for s in range(S):
-        for t in range(T):
-            p = starts[s] + t
-            if starts[s] < 0 or starts[s] >= limit or p >= limit:
-                continue
-            for g in range(KV):
-                kk = np.concatenate([pk[g], k[s, g, :p + 1]]).astype(np.float64)
-                vv = np.concatenate([pv[g], v[s, g, :p + 1]]).astype(np.float64)
-                hs = slice(g * H // KV, (g + 1) * H // KV)
-                sc = q[s, t, hs] @ kk.T / math.sqrt(hd)
-                w = np.exp(sc - sc.max(-1, keepdims=True))
-                w /= w.sum(-1, keepdims=True)
-                out[s, t, hs], scale[s, t, hs] = w @ vv, w @ np.abs(vv)
-                total[s, t, hs] = np.abs(vv).sum(0)
-                size[s, t, hs, 0] = (np.abs(q[s, t, hs]) @ np.abs(kk).T).max(-1) / math.sqrt(hd)
+    live = [s for s in range(S) if 0 <= starts[s] < limit]
+    for g in range(KV):
+        hs = slice(g * G, (g + 1) * G)
+        qg = q[:, :, hs].astype(np.float64) / math.sqrt(hd)
+        pkg, pvg = pk[g].astype(np.float64), pv[g].astype(np.float64)
+        sp, ap = qg @ pkg.T, (np.abs(qg) @ np.abs(pkg).T).max(-1, initial=0)
+        for s in live:
+            n = min(T, limit - starts[s])
+            end = starts[s] + n
+            kk, vv = k[s, g, :end].astype(np.float64), v[s, g, :end].astype(np.float64)
+            hide = (np.arange(end)[None] > starts[s] + np.arange(n)[:, None])[:, None]
+            sc = np.concatenate([sp[s, :n], np.where(hide, -np.inf, qg[s, :n] @ kk.T)], -1)
+            w = np.exp(sc - sc.max(-1, keepdims=True))
+            w /= w.sum(-1, keepdims=True)
+            out[s, :n, hs] = w[..., :P] @ pvg + w[..., P:] @ vv
+            scale[s, :n, hs] = w[..., :P] @ np.abs(pvg) + w[..., P:] @ np.abs(vv)
+            total[s, :n, hs] = np.abs(pvg).sum(0) + np.where(hide, 0.0, 1.0) @ np.abs(vv)
+            size[s, :n, hs, 0] = np.maximum(ap[s, :n], np.where(hide, 0, np.abs(qg[s, :n]) @ np.abs(kk).T).max(-1))
     return out, scale, size, total

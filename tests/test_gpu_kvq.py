@@ -267,11 +267,18 @@ ATTENTIONS = [
     (2, 20, 6, 3, 300, [44, -5], None, 64), (40, 2, 16, 2, 513, [7] * 40, 9, 64),
     (2, 1, 4, 2, 0, [-1, -1], None, 64), (3, 1, 4, 2, 70, [-1, -1, -1], None, 64),  # nothing to attend to
 ]
+# enough rows and keys for the forms that share more: 64-row tiles by one key group, 128-row tiles behind long contexts and
+# over long shared prefixes (own rows by 16 and by 32), chunks by the dozen
+LARGE = [
+    (16, 400, 8, 4, 0, [0] * 15 + [3], 640, 640), (4, 70, 16, 8, 0, [3000, 2999, 2950, 17], None, 3136),
+    (400, 1, 8, 8, 6200, [i % 61 - 1 for i in range(400)], None, 64), (40, 5, 32, 8, 3601, list(range(40)), 64, 64),
+    (1, 1, 8, 2, 0, [5000], None, 5056),
+]
 
 
 @pytest.mark.parametrize("ty", TYPES)
 @pytest.mark.parametrize("hd", [64, 128])
-@pytest.mark.parametrize("case", ATTENTIONS)
+@pytest.mark.parametrize("case", ATTENTIONS + LARGE)
 def test_attention(dev, ty, hd, case):
     S, T, H, KV, P, starts, limit, ctx = case
     print(f"[gpu] attn_kvq {ty} {hd} {case}", flush=True)
