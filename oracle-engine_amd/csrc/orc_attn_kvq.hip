@@ -248,8 +248,9 @@ __device__ __forceinline__ float ka_max(float a, float b) { return __builtin_ele
 // Two fp16 halves of a and b. `minus` is -1 where the compiler does not see it, so that the rest is one v_fma_mix_f32
 // (which widens its fp16 factor) instead of a conversion and a subtraction.
 __device__ __forceinline__ uint32_t ka_split(float a, float b, float minus, uint32_t& lo) {
-    const kq_h2 hi = __builtin_bit_cast(kq_h2, __builtin_amdgcn_cvt_pkrtz(a, b));
-    lo = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(__builtin_fmaf((float)hi.x, minus, a), __builtin_fmaf((float)hi.y, minus, b)));
+    const kq_h2 hi = __builtin_convertvector((kq_f2){a, b}, kq_h2);
+    const kq_f2 rest = {__builtin_fmaf((float)hi.x, minus, a), __builtin_fmaf((float)hi.y, minus, b)};
+    lo = __builtin_bit_cast(uint32_t, __builtin_convertvector(rest, kq_h2));
     return __builtin_bit_cast(uint32_t, hi);
 }
 __device__ __forceinline__ float ka_minus() {
