@@ -387,7 +387,8 @@ int orc_rope_table(float* d_rope, int pos0, int n_pos, int rot_dim, double base,
  * to the own rows. rope_off is the length of a shared prefix. Rotated values
  * are exact sums rounded once to fp32. The K and V columns of the QKV rows are
  * left as they are; so are q rows of tokens that are not stored, and every
- * other row of the caches. Rows 16-byte aligned. */
+ * other row of the caches. Apart from d_q = d_qkv nothing may overlap. Rows
+ * 16-byte aligned. */
 #define ORC_ROPE_HALF 0
 #define ORC_ROPE_PAIRS 1
 int orc_kvq_store(int type, const float* d_qkv, int ldqkv, int n_seq, int n_tok, int n_heads, int n_kv, int head_dim,
@@ -397,7 +398,7 @@ int orc_kvq_store(int type, const float* d_qkv, int ldqkv, int n_seq, int n_tok,
 /* Rows start_i .. start_i + n - 1 of every sequence and kv head as fp32,
  * [n_seq][n_kv][n][head_dim]: what the cache stands for, exactly. Rows outside
  * the cache are zeros. K and V in one call; either pair (d_kc, d_k) or (d_vc,
- * d_v) may be null. */
+ * d_v) may be null. n_seq * n_kv at most 65535. */
 int orc_kvq_load(int type, const void* d_kc, const void* d_vc, int n_seq, int n_kv, int head_dim, int ctx,
                  const int32_t* d_pos, int pos_off, int n, float* d_k, float* d_v, orc_stream_t stream);
 
@@ -413,11 +414,13 @@ int orc_kvq_load(int type, const void* d_kc, const void* d_vc, int n_seq, int n_
  * d_pos null, pos_off + n_tok must not exceed pos_limit.
  * q is split in two fp16 halves (22 bits), the weights likewise, the cache's
  * values are fp16 numbers: products are exact, sums fp32, and the error is
- * that of an fp32 evaluation. Results depend on the shape of the call
- * (n_seq, n_tok, prefix_len, pos_limit) in their rounding only. A NaN in a K or
- * V row reaches the tokens that see the row; among the new tokens of one
- * sequence a NaN or infinity in a V row may also reach the ones before it.
- * Contents of rows that no token sees do not matter.
+ * that of an fp32 evaluation (a weight below 2^-29 of the row's largest keeps
+ * fewer bits: 2^-39 of the largest). Results depend on the shape of the call
+ * (n_seq, n_tok, prefix_len, pos_limit) in their rounding only; the same call
+ * gives the same bits. A NaN or infinity in a K or V row makes the tokens that
+ * see the row NaN (in V: the head dims it is in); in a V row of the call's own
+ * tokens it may also reach the tokens of the sequence before it. Contents of
+ * rows that no token sees do not matter.
  * d_work: orc_attn_kvq_workspace() bytes for the same arguments, 16-byte
  * aligned (0 bytes: null); calls that share it must not overlap. */
 size_t orc_attn_kvq_workspace(int n_seq, int n_tok, int n_heads, int n_kv, int head_dim, int prefix_len, int pos_limit);

@@ -627,7 +627,7 @@ extern "C" int orc_kvq_store(int type, const float* d_qkv, int ldqkv, int n_seq,
     if (!d_pos && (pos_off < 0 || (int64_t)pos_off + n_tok > ctx))
         return set_error(ORC_E_INVALID, "kvq_store: positions must fit the cache");
     const int64_t blocks = ((int64_t)n_seq * n_tok * vecs + 3) / 4;
-    if (blocks > 0xffffff00ll / 256) return set_error(ORC_E_INVALID, "kvq_store: too many rows");
+    if (n_tok < kStoreBlocks && blocks > 0xffffff00ll / 256) return set_error(ORC_E_INVALID, "kvq_store: too many rows");
     const StoreArgs a{d_qkv, ldqkv, n_seq, n_tok, n_heads, n_kv, rope_layout, rot_dim, (const float2*)d_rope, rope_off,
                       d_pos, pos_off, d_q, ldq, (uint8_t*)d_kc, (uint8_t*)d_vc, ctx};
     const hipStream_t st = resolve_stream(s);
@@ -644,7 +644,7 @@ extern "C" int orc_kvq_store(int type, const float* d_qkv, int ldqkv, int n_seq,
         });
     else {
         const int mode = rope_layout == ORC_ROPE_PAIRS || !rot_dim ? kRotPairs : rot_dim == head_dim ? kRotHalf : kRotAny;
-        const int nblk = (n_tok + 2 * kKvBlock - 2) / kKvBlock;  // blocks that n_tok rows may touch
+        const int nblk = (int)(((int64_t)n_tok + 2 * kKvBlock - 2) / kKvBlock);  // blocks that n_tok rows may touch
         const int64_t kv = (int64_t)n_seq * 2 * n_kv * nblk, q = (int64_t)n_seq * n_tok * n_heads;
         const int64_t all = kv + (mode == kRotAny ? (q + 3) / 4 : (q * (head_dim / 8) + 255) / 256);
         if (all > 0xffffff00ll / 256) return set_error(ORC_E_INVALID, "kvq_store: too many rows");

@@ -273,6 +273,9 @@ LARGE = [
     (16, 400, 8, 4, 0, [0] * 15 + [3], 640, 640), (4, 70, 16, 8, 0, [3000, 2999, 2950, 17], None, 3136),
     (400, 1, 8, 8, 6200, [i % 61 - 1 for i in range(400)], None, 64), (40, 5, 32, 8, 3601, list(range(40)), 64, 64),
     (1, 1, 8, 2, 0, [5000], None, 5056),
+    # own rows of several blocks a wave beside a prefix's tiles
+    (17, 1, 8, 2, 1000, [37 * i for i in range(17)], None, 640), (4, 3, 28, 4, 200, [600, 331, -1, 63], None, 640),
+    (100, 1, 16, 4, 12300, [3 * i for i in range(100)], None, 320), (25, 5, 16, 4, 12300, [12 * i for i in range(25)], None, 320),
 ]
 
 
@@ -436,3 +439,85 @@ def test_continuations_of_one_prompt(dev, ty, hd, layout):
         starts = np.where(starts >= 0, starts + 1, starts).astype(np.int32)
     dev.check(L.orc_graph_destroy(graph))
     dev.check(L.orc_stream_destroy(s))
+
+
+@pytest.mark.parametrize("T,layout,rot", [(20, orc.ROPE_HALF, 128), (20, orc.ROPE_HALF, 40), (33, orc.ROPE_PAIRS, 128), (2, orc.ROPE_PAIRS, 40)])
+def test_store_in_place_of_every_form(dev, T, layout, rot):
+    rng = np.random.default_rng(T + rot)
+    S, H, KV, hd, ctx = 2, 4, 2, 128, 128
+    qkv = rng.normal(0, 1, (S * T, (H + 2 * KV) * hd)).astype(np.float32)
+    rope = _table(dev, 0, ctx, rot, 1e4)
+    a, b = (Caches(dev, orc.KV_Q4, S, KV, ctx, hd) for _ in range(2))
+    q = a.store(qkv, T, H, rope, rot, layout, [9, 70])
+    y = b.store(qkv, T, H, rope, rot, layout, [9, 70], in_place=True)
+    assert np.array_equal(y[:, :H * hd], q[:, :-4]) and np.array_equal(y[:, H * hd:], qkv[:, H * hd:])
+    assert np.array_equal(a.k.read(np.uint8), b.k.read(np.uint8)) and np.array_equal(a.v.read(np.uint8), b.v.read(np.uint8))
+
+
+@pytest.mark.parametrize("ty", [orc.F16, orc.KV_Q8])
+def test_a_cache_of_more_than_4_gb(dev, ty):
+    """The last rows of the last of three sequences of 2^20 (F16; 8 bits: 2^21) positions, zeros before them: the rows
+    read back, and attention, whose zero keys weigh exp(0) each.
+
+    Bound: as the others', with up to 2^21 / 64 / 64 = 512 blocks added up per chunk at 2^-24 each, in two sums: 6.1e-5.
+    """
+    S, H, KV, hd, T = 3, 8, 8, 128, 3
+    ctx = 1 << (20 if ty == orc.F16 else 21)
+    rng = np.random.default_rng(21)
+    print(f"[gpu] caches of {dev.L.orc_kvq_bytes(ty, S, KV, ctx, hd) / 2 ** 30:.1f} GB", flush=True)
+    c = Caches(dev, ty, S, KV, ctx, hd)
+    assert c.bytes > 4 << 30
+    for b in (c.k, c.v):
+        dev.check(dev.L.orc_fill(b.ptr, 0, c.bytes, None))
+    if ty != orc.F16:  # code 128 is zero; byte 0 of a group whose scale is zero stands for zero too
+        assert not np.any(c.load(4)[0])
+    pos = [-1, -1, ctx - T]
+    qkv = rng.normal(0, 1, (S * T, (H + 2 * KV) * hd)).astype(np.float32)
+    c.store(qkv, T, H, pos=pos)
+    x = qkv.reshape(S, T, H + 2 * KV, hd)[2]
+    k, v = (ref.quantised(ty, x[:, a:a + KV]) for a in (H, H + KV))
+    got_k, got_v = c.load(T + 2, [0, ctx - T - 2, ctx - T - 2])
+    for got, want in ((got_k, k), (got_v, v)):
+        assert _same(got[2, :, 2:].transpose(1, 0, 2), want) and not np.any(got[2, :, :2]) and not np.any(got[:2])
+    q = (x[:, :H] * 3).astype(np.float32)  # the last keys count against 2^20 zeros
+    full = np.zeros((S, T, H, hd), np.float32)
+    full[2] = q
+    got = _attend(dev, c, full, H, T, pos=pos)
+    assert not np.any(got[:2])
+    for t in range(T):
+        for h in range(H):
+            s = (k[:t + 1, h] @ q[t, h].astype(np.float64)) / np.sqrt(hd)
+            n0 = ctx - T
+            m = max(s.max(), 0)
+            w, z = np.exp(s - m), n0 * np.exp(-m)
+            total = w.sum() + z
+            size = (np.abs(k[:t + 1, h]) @ np.abs(q[t, h])).max() / np.sqrt(hd)
+            err = np.abs(got[2, t, h] - w @ v[:t + 1, h] / total)
+            assert np.all(err <= (6.6e-5 + 2.5e-6 * size) * (w @ np.abs(v[:t + 1, h]) / total) + 2.0 ** -39 * np.abs(v[:t + 1, h]).sum(0)), (t, h)
+
+
+def test_calls_on_two_streams_at_once(dev):
+    """Different shapes on two streams, each with a workspace of its own: the bits of the same calls one by one."""
+    rng = np.random.default_rng(30)
+    hd, KV = 128, 2
+    jobs = []
+    for S, T, H, P, starts, ctx in ((9, 1, 8, 900, list(range(9)), 64), (1, 90, 4, 0, [300], 448)):
+        own, _, _ = _filled(dev, orc.KV_Q8, S, KV, ctx, hd, [s + T for s in starts], rng)
+        pre = _filled(dev, orc.KV_Q8, 1, KV, (P + 63) // 64 * 64, hd, [P], rng)[0] if P else None
+        q = rng.normal(0, 1, (S, T, H, hd)).astype(np.float32)
+        want = _attend(dev, own, q, H, T, pre, P, starts, pad=0)
+        s = C.c_void_p()
+        dev.check(dev.L.orc_stream_create(C.byref(s)))
+        size = dev.L.orc_attn_kvq_workspace(S, T, H, KV, hd, P, ctx)
+        jobs.append((s, dev.upload(q), dev.alloc(q.nbytes), dev.alloc(size + 16), dev.upload(np.asarray(starts, np.int32)), want,
+                     (S, T, H, P, ctx, own, pre)))
+    dev.sync()
+    for _ in range(20):
+        for s, q, out, work, pos, _, (S, T, H, P, ctx, own, pre) in jobs:
+            dev.check(dev.L.orc_attn_kvq(orc.KV_Q8, q.ptr, H * hd, S, T, H, KV, hd, pre and pre.k.ptr, pre and pre.v.ptr, P,
+                                         pre.shape[3] if pre else 0, own.k.ptr, own.v.ptr, ctx, pos.ptr, 0, ctx, out.ptr,
+                                         H * hd, work.ptr, s))
+    dev.sync()
+    for s, q, out, work, pos, want, _ in jobs:
+        assert np.array_equal(out.read(np.uint32), want.view(np.uint32).ravel())
+        dev.check(dev.L.orc_stream_destroy(s))
