@@ -418,9 +418,8 @@ int orc_kvq_load(int type, const void* d_kc, const void* d_vc, int n_seq, int n_
  * fewer bits: 2^-39 of the largest). Results depend on the shape of the call
  * (n_seq, n_tok, prefix_len, pos_limit) in their rounding only; the same call
  * gives the same bits. A NaN or infinity in a K or V row makes the tokens that
- * see the row NaN (in V: the head dims it is in); in a V row of the call's own
- * tokens it may also reach the tokens of the sequence before it. Contents of
- * rows that no token sees do not matter.
+ * see the row NaN (an infinity in V: NaN or infinite, in its head dim) and no
+ * others. Contents of rows that no token sees do not matter.
  * d_work: orc_attn_kvq_workspace() bytes for the same arguments, 16-byte
  * aligned (0 bytes: null); calls that share it must not overlap. */
 size_t orc_attn_kvq_workspace(int n_seq, int n_tok, int n_heads, int n_kv, int head_dim, int prefix_len, int pos_limit);

@@ -174,6 +174,65 @@ __device__ __forceinline__ kq_h2 ka_scale_v(uint32_t w, int e, uint32_t sign = 0
     return __builtin_bit_cast(kq_h2, __builtin_amdgcn_perm(0u, w, 0x000C000Cu | (e << 8) | ((e + 1) << 24)) >> 1 ^ sign);
 }
 
+// ── infinities and NaN in V rows that only some of a tile's rows see ─────────
+// A product of the matrix cores takes every row through every key, and 0 times a NaN is one. In the blocks where a call's
+// own tokens see different numbers of keys, such values are taken out of V and noted, as a 64-bit mask of the block's
+// keys for each head dim, and the rows that do see them are made NaN at the end.
+__device__ __forceinline__ bool ka_odd_scales(uint32_t w) {  // a scale byte of all exponent bits among the four?
+    const uint32_t x = ~w & 0xF8F8F8F8u;
+    return (x - 0x01010101u) & ~x & 0x80808080u;
+}
+__device__ __forceinline__ bool ka_odd_halves(uint32_t w) {
+    return (w & 0x7C00u) == 0x7C00u || (w & 0x7C000000u) == 0x7C000000u;
+}
+// Which of the 16 bytes of sc are odd (bit e: byte e); those become 0 (a scale of 0).
+__device__ __forceinline__ uint32_t ka_take_scales(u32x4& sc) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int e = 0; e < 16; ++e)
+        if ((sc[e >> 2] & (0xF8u << (8 * (e & 3)))) == 0xF8u << (8 * (e & 3))) {
+            m |= 1u << e;
+            sc[e >> 2] &= ~(0xFFu << (8 * (e & 3)));
+        }
+    return m;
+}
+// The same for the 16 halves of a dim, v0 and v1 (32 keys each).
+__device__ __forceinline__ uint32_t ka_take_halves(u32x4& v0, u32x4& v1) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+        u32x4& v = e < 8 ? v0 : v1;
+        const int w = (e & 7) >> 1, sh = (e & 1) * 16;
+        if ((v[w] & (0x7C00u << sh)) == 0x7C00u << sh) {
+            m |= 1u << e;
+            v[w] &= ~(0xFFFFu << sh);
+        }
+    }
+    return m;
+}
+// The lane groups' bits (s, q, i) of a dim as a mask of keys s 32 + q 16 + g 4 + i.
+__device__ __forceinline__ void ka_note(uint64_t* list, int dim, uint32_t m, int g) {
+    uint32_t lo = ((m & 15) | (m >> 4 & 15) << 16) << (g * 4), hi = ((m >> 8 & 15) | (m >> 12 & 15) << 16) << (g * 4);
+#pragma unroll
+    for (int d = 16; d < 64; d *= 2) {
+        lo |= __shfl_xor(lo, d, 64);
+        hi |= __shfl_xor(hi, d, 64);
+    }
+    if (g == 0) list[dim] = (uint64_t)hi << 32 | lo;
+}
+// Four dims' values of a row that sees n of the block's keys: NaN where it sees an odd one.
+__device__ __forceinline__ void ka_spoil(kq_f4& o, const uint64_t* list, int n) {
+    const uint64_t sees = n >= 64 ? ~0ull : n <= 0 ? 0 : (1ull << n) - 1;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        if (list[i] & sees) o[i] = __builtin_nanf("");
+}
+// What the workgroup's NW waves noted of up to N blocks (a tile of 128 tokens ends in up to three).
+template <int HD, int N, int NW> struct KaOdd {
+    uint64_t list[N][HD];
+    int any[N][NW];
+};
+
 // V bytes of one dim tile (both tiles of a pair for 4 bits) of a lane.
 template <int TY, int HD> struct KaV {
     static constexpr int kN = TY == ORC_F16 ? HD / 8 : TY == ORC_KV_Q8 ? HD / 16 : HD / 32;
@@ -219,6 +278,35 @@ template <int TY, int HD> struct KaV {
                     for (int g = 0; g < HD / 32; ++g) sc[g][s * 2 + q] &= m;
                 }
             }
+    }
+    __device__ __forceinline__ bool odd() const {
+        bool any = false;
+        if constexpr (TY == ORC_F16) {
+#pragma unroll
+            for (int i = 0; i < kN; ++i)
+#pragma unroll
+                for (int w = 0; w < 4; ++w) any |= ka_odd_halves(r[i][w]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < HD / 32; ++i)
+#pragma unroll
+                for (int w = 0; w < 4; ++w) any |= ka_odd_scales(sc[i][w]);
+        }
+        return any;
+    }
+    __device__ __forceinline__ void take(uint64_t* list, int lane) {
+        const int c = lane & 15, g = lane >> 4;
+#pragma unroll
+        for (int dt = 0; dt < HD / 16; ++dt) {
+            uint32_t m;
+            if constexpr (TY == ORC_F16) m = ka_take_halves(r[dt * 2], r[dt * 2 + 1]);
+            else {
+                if (dt & 1) continue;
+                m = ka_take_scales(sc[dt / 2]);
+                ka_note(list, (dt + 1) * 16 + c, m, g);
+            }
+            ka_note(list, dt * 16 + c, m, g);
+        }
     }
     // operand of dim tile dt and the 32 keys of step s
     __device__ __forceinline__ kq_h8 op(int dt, int s) const {
@@ -399,6 +487,7 @@ template <int BB> struct KaKeys {
 template <int HD, int RT, int NW> struct KaStreamLds {
     float o[NW][16 * RT][HD + 4];
     float2 ml[NW][16 * RT];
+    KaOdd<HD, 2, NW> odd;
 };
 
 template <int TY, int HD, int RT, int NW>
@@ -415,7 +504,8 @@ __device__ __forceinline__ void ka_stream(const KaArgs& a, KaJob j, KaStreamLds<
     const bool direct = a.cp + a.co == 1;
     if (j.b0 >= j.b1 && !direct) return;
     const KaKeys<BB> keys(a, j);
-    const int least = keys.sees(a.by_group(j.r0));  // what the first row sees
+    const int least = keys.sees(a.by_group(j.r0)), most = keys.sees(a.by_group(j.r1 - 1));  // what the first and last row see
+    if (lane < 2) sh.odd.any[lane][wave] = 0;
     KaK<TY, HD> kr[4] = {};
     KaV<TY, HD> vr = {};
     uint32_t ks = 0;
@@ -489,6 +579,11 @@ __device__ __forceinline__ void ka_stream(const KaArgs& a, KaJob j, KaStreamLds<
         }
         if (lim < kKvBlock) vr.keep(lim, lane);
         vr.pin();
+        if (!pre && least < most && least - key0 < kKvBlock && __ballot(vr.odd())) {
+            vr.take(sh.odd.list[b - (least >> 6)], lane);
+            if (lane == 0) sh.odd.any[b - (least >> 6)][wave] = 1;
+            vr.pin();
+        }
         sgn = -sgn;
         const uint32_t sign = sgn < 0.f ? 0x80008000u : 0u;
         u32x4 ph[RT][2], pl[RT][2];
@@ -547,6 +642,13 @@ __device__ __forceinline__ void ka_stream(const KaArgs& a, KaJob j, KaStreamLds<
             v += *(const kq_f4*)&sh.o[w][rr][d];
         }
         const int tok = a.by_group(row), head = j.kv * a.group + (row - tok * a.group);
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+            int any = 0;
+#pragma unroll
+            for (int w = 0; w < NW; ++w) any |= sh.odd.any[n][w];
+            if (any) ka_spoil(v, sh.odd.list[n] + d, keys.sees(tok) - (((least >> 6) + n) << 6));
+        }
         if (direct) {
             const bool live = j.start >= 0 && j.start + (int64_t)(tok - j.seq * a.n_tok) < a.limit;
             const float inv = (TY == ORC_F16 ? 1.f : 0.0625f) / l;
@@ -605,6 +707,30 @@ template <int TY, int HD> struct KaStage {
                     vs[s * 2 + q] &= m >= 4 ? ~0u : (1u << (8 * m)) - 1u;
             }
     }
+    __device__ __forceinline__ bool odd() const {
+        bool any = false;
+        if constexpr (TY == ORC_F16) {
+#pragma unroll
+            for (int i = 0; i < DW * 2; ++i)
+#pragma unroll
+                for (int w = 0; w < 4; ++w) any |= ka_odd_halves(v[i][w]);
+        } else {
+#pragma unroll
+            for (int w = 0; w < 4; ++w) any |= ka_odd_scales(vs[w]);
+        }
+        return any;
+    }
+    __device__ __forceinline__ void take(uint64_t* list, int wave, int lane) {
+        const int c = lane & 15, g = lane >> 4;
+        if constexpr (TY == ORC_F16) {
+#pragma unroll
+            for (int i = 0; i < DW; ++i) ka_note(list, (wave * DW + i) * 16 + c, ka_take_halves(v[i * 2], v[i * 2 + 1]), g);
+        } else {
+            const uint32_t m = ka_take_scales(vs);
+#pragma unroll
+            for (int i = 0; i < DW; ++i) ka_note(list, (wave * DW + i) * 16 + c, m, g);
+        }
+    }
     // sign: 0x80008000 negates the block's V
     __device__ __forceinline__ void put(uint8_t* kt, uint8_t* vt, int wave, int lane, uint32_t sign) const {
         kq_h2 sc = {};
@@ -635,12 +761,15 @@ template <int TY, int HD> struct KaStage {
     }
 };
 
-template <int HD, int RT, int KG> union KaTileLds {
-    uint8_t t[KG][2][2][kKvBlock * HD * 2];  // [key group][buffer][K, V]
-    struct {                                 // the second key group's sums
-        float o[HD / 16][4 * RT * 64 * 4];   // [dim tile][wave, row tile, lane, dim]
-        float2 ml[4 * RT * 64];
-    } join;
+template <int HD, int RT, int KG> struct KaTileLds {
+    union {
+        uint8_t t[KG][2][2][kKvBlock * HD * 2];  // [key group][buffer][K, V]
+        struct {                                 // the second key group's sums
+            float o[HD / 16][KG == 1 ? 1 : 4 * RT * 64 * 4];  // [dim tile][wave, row tile, lane, dim]
+            float2 ml[KG == 1 ? 1 : 4 * RT * 64];
+        } join;
+    };
+    KaOdd<HD, 3, 4 * KG> odd;
 };
 
 template <int TY, int HD, int RT, int KG>
@@ -661,11 +790,21 @@ __device__ __forceinline__ void ka_tile(const KaArgs& a, KaJob j, KaTileLds<HD, 
     // ends of the keys that the wave's first and last row see
     const int least = keys.sees(a.by_group(w0)), most = keys.sees(a.by_group(min(w0 + 16 * RT, j.r1) - 1));
     const bool rows = w0 < j.r1;
+    // keys that not all of the tile's rows see lie behind this one
+    const int tile_least = keys.sees(a.by_group(j.r0)), apart = j.seq < 0 || tile_least == keys.sees(a.by_group(j.r1 - 1)) ? 0x7fffffff : tile_least;
+    if (lane < 3) sh.odd.any[lane][kg * 4 + wave] = 0;
     KaStage<TY, HD> sg = {};
     auto load = [&](int b) { sg.load(keys.k(b), keys.v(b), wave, lane); };
     auto put = [&](int b, int buf) {
         const int lim = keys.limit(b);
         if (lim < kKvBlock) sg.keep(lim, lane);
+        if (b >= keys.nbp && (b + 1) * kKvBlock > apart) {
+            uint64_t* list = sh.odd.list[b - (apart >> 6)];
+            if (__ballot(sg.odd())) {
+                sg.take(list, wave, lane);
+                if (lane == 0) sh.odd.any[b - (apart >> 6)][kg * 4 + wave] = 1;
+            } else if (lane < HD / 4) list[wave * (HD / 4) + lane] = 0;
+        }
         sg.put(sh.t[kg][buf][0], sh.t[kg][buf][1], wave, lane, buf ? 0u : 0x80008000u);
     };
     const float minus = ka_minus();
@@ -782,6 +921,15 @@ __device__ __forceinline__ void ka_tile(const KaArgs& a, KaJob j, KaTileLds<HD, 
         const int row = w0 + r * 16 + c;
         if (row >= j.r1) continue;
         const int tok = a.by_group(row), head = j.kv * a.group + (row - tok * a.group);
+        if (apart != 0x7fffffff)
+            for (int n = 0; n < 3; ++n) {
+                int any = 0;
+#pragma unroll
+                for (int w = 0; w < 4 * KG; ++w) any |= sh.odd.any[n][w];
+                if (!any) continue;
+#pragma unroll
+                for (int d = 0; d < DT; ++d) ka_spoil(o[r][d], sh.odd.list[n] + d * 16 + g * 4, vis[r] - (((apart >> 6) + n) << 6));
+            }
         if (direct) {
             const bool live = j.start >= 0 && j.start + (int64_t)(tok - j.seq * a.n_tok) < a.limit && l != 0.f;
             const float inv = sgn * (TY == ORC_F16 ? 1.f : 0.0625f) / l;
@@ -878,7 +1026,7 @@ template <int HD, int W> __global__ __launch_bounds__(256) void k_attn_kvq_merge
         for (int d = 32; d; d >>= 1) m = fmaxf(m, __shfl_xor(m, d, 64));
         for (int c = lane; c < n; c += 64) {
             const float2 y = get(c);
-            const float e = y.y == 0.f ? 0.f : __builtin_amdgcn_exp2f(y.x - m);
+            const float e = y.y == 0.f ? -1.f : __builtin_amdgcn_exp2f(y.x - m);  // -1: nothing of the row
             if (y.y != 0.f) l += e * y.y;
             if (W == 1 || wave == 0) wt[sub][c] = e;
         }
@@ -891,9 +1039,9 @@ template <int HD, int W> __global__ __launch_bounds__(256) void k_attn_kvq_merge
             if (c0 >= W) ask(c0);
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                const float e = c0 + u * W < n ? wt[sub][c0 + u * W] : 0.f;
+                const float e = c0 + u * W < n ? wt[sub][c0 + u * W] : -1.f;
 #pragma unroll
-                for (int i = 0; i < E; ++i) v[i] += e == 0.f ? 0.f : e * x[u][i];
+                for (int i = 0; i < E; ++i) v[i] += e < 0.f ? 0.f : e * x[u][i];
             }
         }
     }

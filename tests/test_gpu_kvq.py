@@ -297,6 +297,62 @@ def test_attention(dev, ty, hd, case):
     _held(got, *ref.attention(q, pk, pv, k, v, starts, end))
 
 
+# every attention kernel, with tokens of one sequence that see different keys (the last: three blocks of them in a tile)
+ODD = [(1, 5, 3, 1, 0, [61], None, 128), (2, 5, 4, 1, 0, [62, 0], None, 128), (1, 9, 7, 1, 70, [331], None, 512),
+       (16, 400, 8, 4, 0, [0] * 15 + [3], 640, 640), (4, 70, 16, 8, 0, [3000, 2999, 2950, 17], None, 3136),
+       (17, 3, 8, 2, 1000, [20 * i for i in range(17)], None, 384), (4, 3, 28, 4, 200, [600, 331, -1, 63], None, 640),
+       (50, 2, 16, 4, 12300, [3 * i for i in range(50)], None, 320), (25, 5, 16, 4, 12300, [12 * i for i in range(25)], None, 320),
+       (8, 130, 8, 8, 0, [2999, 3000, 3001, 2950, 3040, 3050, 3062, 7], None, 3200)]
+
+
+@pytest.mark.parametrize("ty", TYPES)
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("case", ODD)
+def test_nan_in_a_new_row_reaches_only_the_tokens_that_see_it(dev, ty, hd, case):
+    """NaN and infinities in the V rows of some of the call's own tokens, and NaN in a K row: the tokens before them are as
+    they should be, the ones from there on not finite where the row is not."""
+    S, T, H, KV, P, starts, limit, ctx = case
+    print(f"[gpu] attn_kvq, odd rows {ty} {hd} {case}", flush=True)
+    rng = np.random.default_rng(S * 10000 + T * 100 + P + 1)
+    end, G = limit or ctx, H // KV
+    own, k, v = _filled(dev, ty, S, KV, ctx, hd, [min(s + T, end) if s >= 0 else 0 for s in starts], rng)
+    pre, pk, pv = None, np.zeros((KV, 0, hd)), np.zeros((KV, 0, hd))
+    if P:
+        pre, a, b = _filled(dev, ty, 1, KV, (P + 63) // 64 * 64, hd, [P], rng)
+        pk, pv = a[0, :, :P], b[0, :, :P]
+    q = rng.normal(0, 1, (S, T, H, hd)).astype(np.float32)
+    # row t of sequence s anew: V with NaN (dim 3), an infinity (the last dim) and, in one kv head, K with NaN
+    marks = []
+    for s in range(S):
+        if starts[s] < 0:
+            continue
+        t = int(rng.integers(T))
+        row = np.zeros((1, (1 + 2 * KV) * hd), np.float32)
+        kk, vv = k[s, :, starts[s] + t].copy(), v[s, :, starts[s] + t].copy()
+        vv[0, 3], vv[KV - 1, hd - 1] = np.nan, np.inf
+        if s % 2 and KV > 1:
+            kk[1, 7] = np.nan
+        row[0, hd:] = np.concatenate([kk.ravel(), vv.ravel()])
+        one = [-1] * S
+        one[s] = starts[s] + t
+        own.store(np.repeat(row, S, 0), 1, 1, pos=one)
+        marks.append((s, t))
+    k2, v2 = own.load(ctx)
+    # (the row's other values as the cache now holds them: quantised a second time, they may have moved)
+    want, scale, size, total = ref.attention(q, pk, pv, *(np.nan_to_num(x, posinf=0) for x in (k2, v2)), starts, end)
+    got = _attend(dev, own, q, H, T, pre, P, starts, 0, limit)
+    for s, t in marks:
+        p = starts[s] + t
+        bad = ~np.isfinite(v2[s, :, p])  # [KV][hd]
+        bad |= ~np.isfinite(k2[s, :, p]).all(-1)[:, None]
+        assert bad[0, 3] and bad[KV - 1, hd - 1]
+        bad = np.repeat(bad, G, 0)
+        assert not np.isfinite(got[s, t:][:, bad]).any(), (s, t)  # an infinity: NaN or infinite
+        got[s, t:][:, bad] = want[s, t:][:, bad]
+    assert np.isfinite(got).all()
+    _held(got, want, scale, size, total)
+
+
 @pytest.mark.parametrize("ty", TYPES)
 @pytest.mark.parametrize("amp", [1e-6, 1e-3, 30.0, 3e4])
 def test_attention_of_large_and_small_queries(dev, ty, amp):

@@ -155,15 +155,19 @@ def kernels_of(call, ty, hd, case):
     return [re.sub(r"^_ZN3orc\d+|EEv.*$", "", k) for k in kernels]
 
 
-def test_the_gpu_tests_reach_every_attention_kernel(call):
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("ty", [F16, Q8, Q4])
+def test_the_gpu_tests_reach_every_attention_kernel(call, ty, hd):
     """Row tiles of 16, 32, 64 (one and two key groups) and 128, the launches that mix two of them, both merges: for
-    every type and head size."""
+    every type and head size, and all but the merges with tokens that see different keys."""
     import test_gpu_kvq as t
 
-    for ty in t.TYPES:
-        for hd in (64, 128):
-            got = {k.split("I", 1)[0] + " " + ",".join(re.findall(r"Li(\d+)", k)[2 if "merge" not in k else 1:])
-                   for case in t.ATTENTIONS + t.LARGE for k in kernels_of(call, ty, hd, case)}
-            assert got == {"k_attn_kvq 1", "k_attn_kvq 2", "k_attn_kvq_tile 1,1", "k_attn_kvq_tile 1,2", "k_attn_kvq_tile 2,1",
-                           "k_attn_kvq_both 1,1", "k_attn_kvq_both 1,2", "k_attn_kvq_both 2,1", "k_attn_kvq_both 2,2",
-                           "k_attn_kvq_merge 1", "k_attn_kvq_merge 4"}, (ty, hd, got)
+    def reached(cases):
+        return {k.split("I", 1)[0] + " " + ",".join(re.findall(r"Li(\d+)", k)[2 if "merge" not in k else 1:])
+                for case in cases for k in kernels_of(call, ty, hd, case)}
+
+    main = {"k_attn_kvq 1", "k_attn_kvq 2", "k_attn_kvq_tile 1,1", "k_attn_kvq_tile 1,2", "k_attn_kvq_tile 2,1",
+            "k_attn_kvq_both 1,1", "k_attn_kvq_both 1,2", "k_attn_kvq_both 2,1", "k_attn_kvq_both 2,2"}
+    merges = {"k_attn_kvq_merge 1", "k_attn_kvq_merge 4"}
+    assert reached(t.ATTENTIONS + t.LARGE) == main | merges
+    assert reached(t.ODD) >= main
