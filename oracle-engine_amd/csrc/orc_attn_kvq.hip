@@ -13,6 +13,19 @@
 // block's weights are negated, so that what is left of that drift cancels.
 // The weights carry 2^15 (they cancel against their sum), which keeps both
 // halves normal fp16 numbers down to weights of 2^-29.
+// How the work is cut (ka_plan): the rows of one kv head, tokens times the
+// query heads of its group, in tiles of 16 or 32 (k_attn_kvq: the waves share
+// out the keys), 64 or 128 (k_attn_kvq_tile: the waves share the keys'
+// operands); the keys in chunks where the tiles alone leave CUs idle, merged by
+// k_attn_kvq_merge. With a shared prefix its jobs take the rows of all
+// sequences, so the prefix is read once per row tile and not per sequence, and
+// the own rows are chunks of their own in the same launch (k_attn_kvq_both).
+// Bounds: few rows are bound by latency (a launch's first load is 1 us away, a
+// block of 64 keys takes a wave 1.2 us alone) or by the cache's bytes (64
+// sequences of 4000 rows, 8 kv heads of 128, 8 bits: 5.5 TB/s), many rows by
+// the matrix and vector instructions together, which hardly overlap on this
+// card (a 16x16x32 product and four fp32 multiply-adds, four waves a SIMD:
+// 11.7 ns against 8.7 and 4.4 alone).
 #include "orc_kvq.hpp"
 
 #include <algorithm>
@@ -483,7 +496,11 @@ template <int BB> struct KaKeys {
 
 // ── few rows: the waves share out the keys ───────────────────────────────────
 // A workgroup takes 16 RT rows; its NW waves take every NW-th key block each,
-// straight from memory to operands, and join their sums at the end.
+// straight from memory to operands, and join their sums at the end. The loads
+// of a wave are whole KB in a row, and no key is read twice. Decode of 64
+// sequences at 4000 (32/8 heads of 128): 8 bits 99 us, 5.5 TB/s; fp16, 32 of
+// them, 97 us, 5.4 TB/s; 4 bits 74 us, 3.8 TB/s (there the conversions take as
+// long as the bytes). One token at 300: 6.2 us, most of it latency.
 template <int HD, int RT, int NW> struct KaStreamLds {
     float o[NW][16 * RT][HD + 4];
     float2 ml[NW][16 * RT];
@@ -668,7 +685,15 @@ __device__ __forceinline__ void ka_stream(const KaArgs& a, KaJob j, KaStreamLds<
 // chunk. Each wave turns a quarter of the block into operands in LDS (two
 // buffers, one barrier per block), the next block's bytes are on their way
 // meanwhile: the conversion costs a quarter of what it would in each wave, and
-// an operand read serves 2 RT products.
+// an operand read serves 2 RT products. KG = 2: two such groups of waves take
+// alternate blocks of one row tile and join their sums in LDS, where the rows
+// are too few to fill the card (500 tokens, 32/8 heads of 128: 28 -> 16 us; at
+// 2000 tokens it would cost 82 -> 94). RT = 2 shares more (4000 tokens: 286 ->
+// 237 us), RT = 1 spreads a prompt over more CUs (2047 tokens of 64-wide heads:
+// 56 -> 47). 48 x 4 tokens over a 32 K prompt: 179 us, 1030 TFLOP/s of products
+// with both halves, against 1156 of an 8192 x 8192 x 8192 library product.
+// Forming the next block's scores beside this block's weights was 2-8 % slower,
+// with and without an interleaving asked of the compiler.
 template <int TY, int HD> struct KaStage {
     static constexpr int DW = HD / 64;  // dim tiles of V a wave stages
     KaK<TY, HD> k;
@@ -977,7 +1002,8 @@ template <int TY, int HD, int RP, int RO> __global__ __launch_bounds__(256, 2) v
 // ── the chunks' partial sums ─────────────────────────────────────────────────
 // out = sum over chunks of 2^(m_c - max) O_c over the same of l_c, W waves a
 // row: the lanes form the chunks' weights side by side, then each wave adds
-// every W-th chunk.
+// every W-th chunk. Bound by two latencies, the sums' and, asked for with them,
+// the rows': 4.3 us for 252 rows of 33 chunks.
 constexpr int kKaSlots = 1024;
 template <int HD, int W> __global__ __launch_bounds__(256) void k_attn_kvq_merge(KaArgs a, float unit) {
     constexpr int R = 4 / W, E = HD / 64, N = W == 1 ? 16 : kKaSlots;  // rows of a workgroup
