@@ -397,8 +397,9 @@ int orc_kvq_store(int type, const float* d_qkv, int ldqkv, int n_seq, int n_tok,
 
 /* Rows start_i .. start_i + n - 1 of every sequence and kv head as fp32,
  * [n_seq][n_kv][n][head_dim]: what the cache stands for, exactly. Rows outside
- * the cache are zeros. K and V in one call; either pair (d_kc, d_k) or (d_vc,
- * d_v) may be null. n_seq * n_kv at most 65535. */
+ * 0..ctx-1 are zeros (a start may be negative here). K and V in one call;
+ * either pair (d_kc, d_k) or (d_vc, d_v) may be null. n_seq * n_kv at most
+ * 65535. */
 int orc_kvq_load(int type, const void* d_kc, const void* d_vc, int n_seq, int n_kv, int head_dim, int ctx,
                  const int32_t* d_pos, int pos_off, int n, float* d_k, float* d_v, orc_stream_t stream);
 

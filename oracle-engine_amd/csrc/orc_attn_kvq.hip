@@ -1199,7 +1199,7 @@ extern "C" int orc_attn_kvq(int type, const float* d_q, int ldq, int n_seq, int 
           (uintptr_t)d_work) & 15))
         return set_error(ORC_E_INVALID, "attn_kvq: null or misaligned pointer");
     const int64_t jobs_p = (int64_t)n_kv * p.cp * p.tiles_p, jobs_o = (int64_t)n_seq * n_kv * p.co * p.tiles_o;
-    if (jobs_p + jobs_o > 0xffffff00ll / 256 - 16) return set_error(ORC_E_INVALID, "attn_kvq: too many rows");
+    if (jobs_p + jobs_o > 0xffffff00ll / 256 - 16 || (p.slots() > 1 && p.rows > 4 * (0xffffff00ull / 256))) return set_error(ORC_E_INVALID, "attn_kvq: too many rows");
     KaArgs a{d_q, ldq, n_seq, n_tok, n_heads, n_kv, n_heads / n_kv, (const uint8_t*)d_pk, (const uint8_t*)d_pv,
              (const uint8_t*)d_kc, (const uint8_t*)d_vc, prefix_len, prefix_ctx, ctx, d_pos, pos_off, pos_limit, d_out,
              ldo, nullptr, nullptr, (int)p.rows, p.shared, p.tiles_p, p.cp, p.tiles_o, p.co, (int)jobs_p, (int)jobs_o,

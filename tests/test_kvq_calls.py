@@ -125,7 +125,7 @@ def attn(type=Q8, q=1, ldq=None, ns=2, nt=3, h=4, kv=2, hd=64, pk=1, pv=1, pl=10
     ({"ldo": 257}, INVALID), ({"ns": -1}, INVALID), ({"nt": -2}, INVALID), ({"h": 5}, INVALID), ({"kv": 0}, INVALID),
     ({"h": 0}, INVALID), ({"pl": 129}, INVALID), ({"pl": -1}, INVALID), ({"pc": 100}, INVALID), ({"ctx": 130, "lim": 100}, INVALID),
     ({"lim": 0}, INVALID), ({"lim": 129}, INVALID), ({"pos": 0, "off": 126}, INVALID), ({"pos": 0, "off": -1}, INVALID),
-    ({"ns": 1 << 15, "nt": 1 << 15}, INVALID), ({"nt": 1 << 25, "ctx": 0x7fffff00 - 192, "lim": 0x7fffff00 - 192}, INVALID)])
+    ({"ns": 1 << 15, "nt": 1 << 15}, INVALID), ({"ns": 1 << 22, "nt": 1, "h": 32, "kv": 1}, INVALID), ({"nt": 1 << 25, "ctx": 0x7fffff00 - 192, "lim": 0x7fffff00 - 192}, INVALID)])
 def test_attention_refuses(call, args, code):
     rc, kernels, msg = call(attn(**args))[0]
     assert rc == code and not kernels and msg.startswith("attn_kvq")
