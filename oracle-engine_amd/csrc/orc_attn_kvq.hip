@@ -1136,8 +1136,11 @@ static KaPlan ka_plan(int n_seq, int n_tok, int n_heads, int n_kv, int hd, int p
         if (p.m_o == 64 && (int64_t)n_seq * n_kv * ka_div(rows_o, 64) * ka_div(nbp + nbo, 4) < 2048) p.kg = 2;
     }
     p.tiles_o = ka_div(rows_o, p.m_o);
-    const int64_t base_o = (int64_t)n_seq * n_kv * p.tiles_o, fill = 512 / p.kg;  // workgroups that fill the card
-    p.co = ka_chunks(base_o, p.shared ? nbo : nbp + nbo, fill, p.m_o <= 32 ? 12 : 4 * p.kg);
+    // Workgroups that fill the card: two a CU where tiles are multiplied, one where K and V stream past few rows (a
+    // second adds no bandwidth but partial sums: 32000 tokens, 32/8 heads of 128, 8 bits: 23.9 us with 512, 19.3 with
+    // 256; 16 sequences x 4 tokens of 4000, 28/4 heads: 33.6 and 27.7; but 512 tokens after 7500: 135 and 178).
+    const int64_t base_o = (int64_t)n_seq * n_kv * p.tiles_o, fill = 512 / p.kg;
+    p.co = ka_chunks(base_o, p.shared ? nbo : nbp + nbo, p.m_o <= 32 ? 256 : fill, p.m_o <= 32 ? 12 : 4 * p.kg);
     if (p.shared) {
         p.tiles_p = ka_div(rows_p, p.m_p);
         const int64_t base_p = (int64_t)n_kv * p.tiles_p;
