@@ -499,7 +499,7 @@ template <int BB> struct KaKeys {
 // straight from memory to operands, and join their sums at the end. The loads
 // of a wave are whole KB in a row, and no key is read twice. Decode of 64
 // sequences at 4000 (32/8 heads of 128): 8 bits 99 us, 5.5 TB/s; fp16, 32 of
-// them, 97 us, 5.4 TB/s; 4 bits 74 us, 3.8 TB/s (there the conversions take as
+// them, 90 us, 5.8 TB/s; 4 bits 71 us, 4.0 TB/s (there the conversions take as
 // long as the bytes). One token at 300: 6.2 us, most of it latency.
 template <int HD, int RT, int NW> struct KaStreamLds {
     float o[NW][16 * RT][HD + 4];
