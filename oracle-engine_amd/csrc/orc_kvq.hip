@@ -558,7 +558,9 @@ using namespace orc;
 extern "C" size_t orc_kvq_bytes(int type, int n_seq, int n_kv, int ctx, int head_dim) {
     if (!kvq_type_ok(type) || (head_dim != 64 && head_dim != 128) || n_seq < 1 || n_kv < 1 || ctx < 1 || ctx % kKvBlock)
         return 0;
-    return (size_t)n_seq * n_kv * (ctx / kKvBlock) * kvq_block_bytes(type, head_dim);
+    size_t bytes = (size_t)n_seq * n_kv;  // below 2^62
+    if (__builtin_mul_overflow(bytes, (size_t)(ctx / kKvBlock) * kvq_block_bytes(type, head_dim), &bytes)) return 0;
+    return bytes;
 }
 
 extern "C" int orc_rope_table(float* d_rope, int pos0, int n_pos, int rot_dim, double base,
@@ -632,7 +634,9 @@ extern "C" int orc_kvq_store(int type, const float* d_qkv, int ldqkv, int n_seq,
     if (d_q == d_qkv && ldq != ldqkv) return set_error(ORC_E_INVALID, "kvq_store: q in place needs ldq = ldqkv");
     if (!d_pos && (pos_off < 0 || (int64_t)pos_off + n_tok > ctx))
         return set_error(ORC_E_INVALID, "kvq_store: positions must fit the cache");
-    const int64_t blocks = ((int64_t)n_seq * n_tok * vecs + 3) / 4;
+    const int64_t rows = (int64_t)n_seq * n_tok;
+    if (rows > 0x7fffffff) return set_error(ORC_E_INVALID, "kvq_store: too many rows");
+    const int64_t blocks = (rows * vecs + 3) / 4;
     if (n_tok < kStoreBlocks && blocks > 0xffffff00ll / 256) return set_error(ORC_E_INVALID, "kvq_store: too many rows");
     const StoreArgs a{d_qkv, ldqkv, n_seq, n_tok, n_heads, n_kv, rope_layout, rot_dim, (const float2*)d_rope, rope_off,
                       d_pos, pos_off, d_q, ldq, (uint8_t*)d_kc, (uint8_t*)d_vc, ctx};
@@ -651,7 +655,7 @@ extern "C" int orc_kvq_store(int type, const float* d_qkv, int ldqkv, int n_seq,
     else {
         const int mode = rope_layout == ORC_ROPE_PAIRS || !rot_dim ? kRotPairs : rot_dim == head_dim ? kRotHalf : kRotAny;
         const int nblk = (int)(((int64_t)n_tok + 2 * kKvBlock - 2) / kKvBlock);  // blocks that n_tok rows may touch
-        const int64_t kv = (int64_t)n_seq * 2 * n_kv * nblk, q = (int64_t)n_seq * n_tok * n_heads;
+        const int64_t kv = (int64_t)n_seq * 2 * n_kv * nblk, q = rows * n_heads;
         const int64_t all = kv + (mode == kRotAny ? (q + 3) / 4 : (q * (head_dim / 8) + 255) / 256);
         if (all > 0xffffff00ll / 256) return set_error(ORC_E_INVALID, "kvq_store: too many rows");
         each([&](auto ty, auto hd) {

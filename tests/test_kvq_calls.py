@@ -78,7 +78,8 @@ def store(type=Q8, qkv=1, ld=None, ns=2, nt=3, h=4, kv=2, hd=64, lay=0, rot=64, 
     ({"nt": -1}, INVALID), ({"h": 0}, INVALID), ({"kv": 0}, INVALID), ({"lay": 2}, INVALID), ({"rot": 63}, INVALID),
     ({"rot": 66}, INVALID), ({"rot": -2}, INVALID), ({"ro": -1}, INVALID), ({"ctx": 0}, INVALID), ({"ctx": 100}, INVALID),
     ({"pos": 0, "off": 126}, INVALID), ({"pos": 0, "off": -1}, INVALID), ({"q": 3}, INVALID),
-    ({"ns": 1 << 15, "nt": 1 << 15, "ctx": 1 << 15}, INVALID)])
+    ({"ns": 1 << 15, "nt": 1 << 15, "ctx": 1 << 15}, INVALID), ({"ns": 1 << 30, "nt": 1 << 30, "ctx": 1 << 30}, INVALID),
+    ({"ns": 0x7fffffff, "nt": 15}, INVALID)])
 def test_store_refuses(call, args, code):
     rc, kernels, msg = call(store(**args))[0]
     assert rc == code and not kernels and msg.startswith("kvq_store")
@@ -139,8 +140,10 @@ def test_sizes(call):
     got = [c[0] for c in call(["bytes", F16, 3, 2, 128, 64], ["bytes", Q8, 3, 2, 128, 64], ["bytes", Q4, 1, 4, 64, 128],
                               ["bytes", 8, 1, 1, 64, 64], ["bytes", Q8, 1, 1, 100, 64], ["bytes", Q8, 1, 1, 64, 96],
                               ["bytes", Q8, 0, 1, 64, 64], ["bytes", Q8, 1, 0, 64, 64], ["bytes", Q8, 1, 1, 0, 64],
-                              ["bytes", Q8, 64, 8, 1 << 20, 128])]
-    assert got == [3 * 2 * 128 * 128, 3 * 2 * 128 * 66, 4 * 64 * 68, 0, 0, 0, 0, 0, 0, 64 * 8 * (1 << 20) * 132]
+                              ["bytes", Q8, 64, 8, 1 << 20, 128],
+                              ["bytes", F16, 0x7fffffff, 0x7fffffff, 128, 64])]
+    # the last one's product passes 64 bits
+    assert got == [3 * 2 * 128 * 128, 3 * 2 * 128 * 66, 4 * 64 * 68, 0, 0, 0, 0, 0, 0, 64 * 8 * (1 << 20) * 132, 0]
     # no workspace where one chunk holds all; none for shapes that a call would refuse
     got = [c[0] for c in call(["work", 1, 1, 14, 2, 64, 0, 300], ["work", 1, 1, 5, 2, 64, 0, 300], ["work", 1, 1, 4, 2, 96, 0, 300],
                               ["work", 2, 1, 4, 2, 64, 100, 64])]
