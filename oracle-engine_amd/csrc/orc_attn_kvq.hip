@@ -33,16 +33,6 @@
 
 namespace orc {
 
-// Division of a non-negative int by one that the host knows: a product and a shift instead of the 40 instructions of a
-// quotient of two registers, which stood between a workgroup's start and its first load.
-struct KaDiv {
-    uint32_t mul;  // 2^(31 + shift) / d rounded down, and 1
-    int shift, d;
-    __device__ __forceinline__ int operator()(int n) const {
-        return d == 1 ? n : (int)(__umulhi((uint32_t)n << 1, mul) >> shift);
-    }
-};
-
 struct KaArgs {
     const float* q;
     int ldq, n_seq, n_tok, n_heads, n_kv, group;
@@ -58,11 +48,11 @@ struct KaArgs {
     // jobs: prefix ones (shared form only), then own ones
     int shared, tiles_p, cp, tiles_o, co;
     int jobs_p, jobs_o;
-    KaDiv by_group, by_kv, by_tiles_p, by_cp, by_tiles_o, by_co, by_heads, by_tok;
+    KvqDiv by_group, by_kv, by_tiles_p, by_cp, by_tiles_o, by_co, by_heads, by_tok;
 };
 
 // Blocks [b0, b1) of chunk c of n chunks over nb blocks.
-__device__ __forceinline__ void ka_chunk(int nb, const KaDiv& n, int c, int& b0, int& b1) {
+__device__ __forceinline__ void ka_chunk(int nb, const KvqDiv& n, int c, int& b0, int& b1) {
     const int per = n(nb + n.d - 1);
     b0 = min(nb, c * per);
     b1 = min(nb, b0 + per);
@@ -1098,13 +1088,6 @@ struct KaPlan {
     size_t bytes(int hd) const { return slots() > 1 ? (size_t)slots() * rows * (4 * (size_t)hd + 8) : 0; }
 };
 
-static KaDiv ka_fast(int d) {
-    KaDiv r{0, 0, std::max(d, 1)};
-    while (((int64_t)1 << r.shift) < r.d) ++r.shift;
-    if (r.d > 1) r.mul = (uint32_t)((((uint64_t)1 << (31 + r.shift)) / r.d) + 1);
-    return r;
-}
-
 static int ka_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 
 // Chunks of nb key blocks for `base` workgroups' worth of row tiles: at most `most` workgroups, and four blocks each or
@@ -1206,8 +1189,8 @@ extern "C" int orc_attn_kvq(int type, const float* d_q, int ldq, int n_seq, int 
     KaArgs a{d_q, ldq, n_seq, n_tok, n_heads, n_kv, n_heads / n_kv, (const uint8_t*)d_pk, (const uint8_t*)d_pv,
              (const uint8_t*)d_kc, (const uint8_t*)d_vc, prefix_len, prefix_ctx, ctx, d_pos, pos_off, pos_limit, d_out,
              ldo, nullptr, nullptr, (int)p.rows, p.shared, p.tiles_p, p.cp, p.tiles_o, p.co, (int)jobs_p, (int)jobs_o,
-             ka_fast(n_heads / n_kv), ka_fast(n_kv), ka_fast(p.tiles_p), ka_fast(p.cp), ka_fast(p.tiles_o), ka_fast(p.co),
-             ka_fast(n_heads), ka_fast(n_tok)};
+             kvq_div(n_heads / n_kv), kvq_div(n_kv), kvq_div(p.tiles_p), kvq_div(p.cp), kvq_div(p.tiles_o), kvq_div(p.co),
+             kvq_div(n_heads), kvq_div(n_tok)};
     if (bytes) {
         a.part_o = (float*)d_work;
         a.part_ml = (float2*)((uint8_t*)d_work + (size_t)p.slots() * p.rows * head_dim * 4);

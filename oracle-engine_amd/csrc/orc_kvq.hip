@@ -76,6 +76,7 @@ struct StoreArgs {
     int ldq;
     uint8_t *kc, *vc;
     int ctx;
+    KvqDiv by_vecs, by_tok, by_heads;
 };
 
 // Rotated value d of the head vector x. The products of two fp32 numbers are
@@ -106,15 +107,13 @@ __device__ __forceinline__ float kvq_rotated(const float* x, int d, int layout, 
 // 3.5 us for one token, 4.6 us for 61 of 32/8 heads.
 template <int TY, int HD> __global__ __launch_bounds__(256) void k_kvq_store(StoreArgs a) {
     const int lane = threadIdx.x & 63;
-    const int64_t unit = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    const int vecs = a.n_heads + 2 * a.n_kv;
-    const int64_t row = unit / vecs;
-    if (row >= (int64_t)a.n_seq * a.n_tok) return;
-    const int h = (int)(unit - row * vecs), seq = (int)(row / a.n_tok), t = (int)(row - (int64_t)seq * a.n_tok);
+    const int unit = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), row = a.by_vecs(unit);
+    if (row >= a.n_seq * a.n_tok) return;
+    const int h = unit - row * a.by_vecs.d, seq = a.by_tok(row), t = row - seq * a.n_tok;
     const int start = kvq_start(a.d_pos, seq, a.pos_off, a.ctx);
     if (start < 0 || start + (int64_t)t >= a.ctx) return;
     const int p = start + t;
-    const float* x = a.qkv + row * a.ldqkv + (size_t)h * HD;
+    const float* x = a.qkv + (int64_t)row * a.ldqkv + (size_t)h * HD;
     const float2* cs = a.rope + (a.rope_off + p) * (a.rot >> 1);
     const bool is_v = h >= a.n_heads + a.n_kv;
     constexpr int E = HD / 64;
@@ -122,7 +121,7 @@ template <int TY, int HD> __global__ __launch_bounds__(256) void k_kvq_store(Sto
 #pragma unroll
     for (int e = 0; e < E; ++e) v[e] = kvq_rotated(x, lane + 64 * e, a.layout, is_v ? 0 : a.rot, cs);
     if (h < a.n_heads) {
-        float* q = a.q + row * a.ldq + (size_t)h * HD;
+        float* q = a.q + (int64_t)row * a.ldq + (size_t)h * HD;
 #pragma unroll
         for (int e = 0; e < E; ++e) q[lane + 64 * e] = v[e];
         return;
@@ -361,16 +360,14 @@ __device__ __forceinline__ void kvq_store_v(const StoreArgs& a, int seq, int kv,
 }
 
 // eight values of a q vector a thread: four and the four HD / 2 further on, or eight in a row
-template <int HD> __device__ __forceinline__ void kvq_store_q(const StoreArgs& a, int mode, int64_t it) {
-    const int part = (int)(it % (HD / 8));
-    const int64_t hv = it / (HD / 8), row = hv / a.n_heads;
-    if (row >= (int64_t)a.n_seq * a.n_tok) return;
-    const int h = (int)(hv - row * a.n_heads), seq = (int)(row / a.n_tok);
-    const int start = kvq_start(a.d_pos, seq, a.pos_off, a.ctx);
-    const int64_t p = start + (row - (int64_t)seq * a.n_tok);
+template <int HD> __device__ __forceinline__ void kvq_store_q(const StoreArgs& a, int mode, int w) {
+    const int part = threadIdx.x % (HD / 8), hv = w * (256 / (HD / 8)) + threadIdx.x / (HD / 8), row = a.by_heads(hv);
+    if (row >= a.n_seq * a.n_tok) return;
+    const int h = hv - row * a.n_heads, seq = a.by_tok(row), start = kvq_start(a.d_pos, seq, a.pos_off, a.ctx);
+    const int64_t p = (int64_t)start + (row - seq * a.n_tok);
     if (start < 0 || p >= a.ctx) return;
-    const float* x = a.qkv + row * a.ldqkv + (size_t)h * HD;
-    float* q = a.q + row * a.ldq + (size_t)h * HD;
+    const float* x = a.qkv + (int64_t)row * a.ldqkv + (size_t)h * HD;
+    float* q = a.q + (int64_t)row * a.ldq + (size_t)h * HD;
     const float2* cs = a.rope + (a.rope_off + p) * (a.rot >> 1);
     const int d0 = mode == kRotPairs ? part * 8 : part * 4, d1 = mode == kRotPairs ? d0 + 4 : d0 + HD / 2;
     kq_f4 v0 = *(const kq_f4*)(x + d0), v1 = *(const kq_f4*)(x + d1);
@@ -406,11 +403,11 @@ template <int HD> __device__ __forceinline__ void kvq_store_q(const StoreArgs& a
 // Grid: blocks_kv workgroups of K and V blocks (nblk a sequence and head), then q. kRotAny's q vectors, whose pairs lie
 // anywhere in the head, take a wave each as in k_kvq_store.
 template <int TY, int HD>
-__global__ __launch_bounds__(256) void k_kvq_store_blocks(StoreArgs a, int mode, int nblk, int64_t blocks_kv) {
+__global__ __launch_bounds__(256) void k_kvq_store_blocks(StoreArgs a, int mode, KvqDiv by_nblk, KvqDiv by_kv2, int blocks_kv) {
     __shared__ StoreLds<TY, HD> sh;
-    int64_t w = blockIdx.x;
+    int w = blockIdx.x;
     if (w < blocks_kv) {
-        const int bi = (int)(w % nblk), kv2 = (int)(w / nblk % (2 * a.n_kv)), seq = (int)(w / nblk / (2 * a.n_kv));
+        const int v = by_nblk(w), bi = w - v * by_nblk.d, seq = by_kv2(v), kv2 = v - seq * by_kv2.d;
         const int start = kvq_start(a.d_pos, seq, a.pos_off, a.ctx);
         const int64_t b = start / kKvBlock + (int64_t)bi;
         if (start < 0 || b >= a.ctx / kKvBlock || b * kKvBlock >= (int64_t)start + a.n_tok) return;
@@ -420,18 +417,16 @@ __global__ __launch_bounds__(256) void k_kvq_store_blocks(StoreArgs a, int mode,
     }
     w -= blocks_kv;
     if (mode != kRotAny) {
-        kvq_store_q<HD>(a, mode, w * 256 + threadIdx.x);
+        kvq_store_q<HD>(a, mode, w);
         return;
     }
-    const int lane = threadIdx.x & 63;
-    const int64_t hv = w * 4 + (threadIdx.x >> 6), row = hv / a.n_heads;
-    if (row >= (int64_t)a.n_seq * a.n_tok) return;
-    const int h = (int)(hv - row * a.n_heads), seq = (int)(row / a.n_tok);
-    const int start = kvq_start(a.d_pos, seq, a.pos_off, a.ctx);
-    const int64_t p = start + (row - (int64_t)seq * a.n_tok);
+    const int lane = threadIdx.x & 63, hv = w * 4 + (threadIdx.x >> 6), row = a.by_heads(hv);
+    if (row >= a.n_seq * a.n_tok) return;
+    const int h = hv - row * a.n_heads, seq = a.by_tok(row), start = kvq_start(a.d_pos, seq, a.pos_off, a.ctx);
+    const int64_t p = (int64_t)start + (row - seq * a.n_tok);
     if (start < 0 || p >= a.ctx) return;
-    const float* x = a.qkv + row * a.ldqkv + (size_t)h * HD;
-    float* q = a.q + row * a.ldq + (size_t)h * HD;
+    const float* x = a.qkv + (int64_t)row * a.ldqkv + (size_t)h * HD;
+    float* q = a.q + (int64_t)row * a.ldq + (size_t)h * HD;
     float v[HD / 64];
 #pragma unroll
     for (int e = 0; e < HD / 64; ++e) v[e] = kvq_rotated(x, lane + 64 * e, a.layout, a.rot, a.rope + (a.rope_off + p) * (a.rot >> 1));
@@ -639,7 +634,8 @@ extern "C" int orc_kvq_store(int type, const float* d_qkv, int ldqkv, int n_seq,
     const int64_t blocks = (rows * vecs + 3) / 4;
     if (n_tok < kStoreBlocks && blocks > 0xffffff00ll / 256) return set_error(ORC_E_INVALID, "kvq_store: too many rows");
     const StoreArgs a{d_qkv, ldqkv, n_seq, n_tok, n_heads, n_kv, rope_layout, rot_dim, (const float2*)d_rope, rope_off,
-                      d_pos, pos_off, d_q, ldq, (uint8_t*)d_kc, (uint8_t*)d_vc, ctx};
+                      d_pos, pos_off, d_q, ldq, (uint8_t*)d_kc, (uint8_t*)d_vc, ctx, kvq_div((int)vecs), kvq_div(n_tok),
+                      kvq_div(n_heads)};
     const hipStream_t st = resolve_stream(s);
     auto each = [&](auto f) {  // f of (type, head size)
         using std::integral_constant;
@@ -660,7 +656,7 @@ extern "C" int orc_kvq_store(int type, const float* d_qkv, int ldqkv, int n_seq,
         if (all > 0xffffff00ll / 256) return set_error(ORC_E_INVALID, "kvq_store: too many rows");
         each([&](auto ty, auto hd) {
             hipLaunchKernelGGL((k_kvq_store_blocks<decltype(ty)::value, decltype(hd)::value>), dim3((unsigned)all), dim3(256), 0, st,
-                               a, mode, nblk, kv);
+                               a, mode, kvq_div(nblk), kvq_div(2 * n_kv), (int)kv);
         });
     }
     ORC_LAUNCH_CHECK();
