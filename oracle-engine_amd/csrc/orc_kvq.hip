@@ -76,7 +76,7 @@ struct StoreArgs {
     int ldq;
     uint8_t *kc, *vc;
     int ctx;
-    KvqDiv by_vecs, by_tok, by_heads;
+    KvqDiv by_vecs, by_tok, by_heads;  // by_heads: what of a token's q vectors one wave or set of threads takes
 };
 
 // Rotated value d of the head vector x. The products of two fp32 numbers are
@@ -104,7 +104,7 @@ __device__ __forceinline__ float kvq_rotated(const float* x, int d, int layout, 
 // A few tokens a sequence: one wave per head vector, q heads are rotated, K
 // heads rotated and quantised, V heads quantised. A scale group is 32 lanes; a
 // row's codes are bytes (K: pieces of 16) all over its block. Bound by latency:
-// 3.5 us for one token, 4.6 us for 61 of 32/8 heads.
+// 3.1 us for one token, 4.2 us for 61 of 32/8 heads.
 template <int TY, int HD> __global__ __launch_bounds__(256) void k_kvq_store(StoreArgs a) {
     const int lane = threadIdx.x & 63;
     const int unit = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), row = a.by_vecs(unit);
@@ -161,7 +161,7 @@ template <int TY, int HD> __global__ __launch_bounds__(256) void k_kvq_store(Sto
 // K: a thread takes HD / 8 dims of one key and the ones HD / 2 further on, a rotate-half pair's two sides, so that the
 // row is read once; its codes are whole 16 or 8 byte pieces of the block, stored in order. V: rows go through LDS,
 // since a stored piece is one dim of 16 keys; pieces that hold rows of other calls are written byte by byte. 4001 tokens
-// of 32/8 heads of 128: 41 us, 4.2 TB/s (a wave per head vector: 87 us); from 16 tokens on, fewer fill no block's pieces.
+// of 32/8 heads of 128: 39 us, 4.3 TB/s (a wave per head vector: 87 us); from 16 tokens on, fewer fill no block's pieces.
 constexpr int kStoreBlocks = 16;  // tokens of a sequence from which on a call takes whole blocks
 enum { kRotHalf, kRotPairs, kRotAny };  // whole heads half-split; pairs (2 i, 2 i + 1), or nothing rotated; the rest
 
@@ -359,45 +359,55 @@ __device__ __forceinline__ void kvq_store_v(const StoreArgs& a, int seq, int kv,
     }
 }
 
-// eight values of a q vector a thread: four and the four HD / 2 further on, or eight in a row
+// Eight values of each of up to four q vectors of a token a thread: four and the four HD / 2 further on, or eight in a
+// row, whose pairs' table entries serve all four.
+constexpr int kQHeads = 4;
 template <int HD> __device__ __forceinline__ void kvq_store_q(const StoreArgs& a, int mode, int w) {
-    const int part = threadIdx.x % (HD / 8), hv = w * (256 / (HD / 8)) + threadIdx.x / (HD / 8), row = a.by_heads(hv);
+    constexpr int N = HD / 8;
+    const int part = threadIdx.x % N, unit = w * (256 / N) + threadIdx.x / N, row = a.by_heads(unit);
     if (row >= a.n_seq * a.n_tok) return;
-    const int h = hv - row * a.n_heads, seq = a.by_tok(row), start = kvq_start(a.d_pos, seq, a.pos_off, a.ctx);
+    const int h0 = unit - row * a.by_heads.d, seq = a.by_tok(row), start = kvq_start(a.d_pos, seq, a.pos_off, a.ctx);
     const int64_t p = (int64_t)start + (row - seq * a.n_tok);
     if (start < 0 || p >= a.ctx) return;
-    const float* x = a.qkv + (int64_t)row * a.ldqkv + (size_t)h * HD;
-    float* q = a.q + (int64_t)row * a.ldq + (size_t)h * HD;
-    const float2* cs = a.rope + (a.rope_off + p) * (a.rot >> 1);
     const int d0 = mode == kRotPairs ? part * 8 : part * 4, d1 = mode == kRotPairs ? d0 + 4 : d0 + HD / 2;
-    kq_f4 v0 = *(const kq_f4*)(x + d0), v1 = *(const kq_f4*)(x + d1);
-    if (mode == kRotHalf) {
+    const float* x = a.qkv + (int64_t)row * a.ldqkv;
+    float* q = a.q + (int64_t)row * a.ldq;
+    const float2* cs = a.rope + (a.rope_off + p) * (a.rot >> 1) + (mode == kRotPairs ? d0 >> 1 : d0);
+    float2 r[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const float2 r = cs[d0 + e];
-            const double va = v0[e], vb = v1[e], co = r.x, si = r.y;
-            v0[e] = (float)(va * co - vb * si);
-            v1[e] = (float)(va * si + vb * co);
-        }
-    } else {
+    for (int e = 0; e < 4; ++e) r[e] = mode == kRotHalf || d0 + 2 * e < a.rot ? cs[e] : make_float2(1.f, 0.f);
+    kq_f4 v0[kQHeads], v1[kQHeads];
 #pragma unroll
-        for (int e = 0; e < 4; e += 2) {
-            if (d0 + e < a.rot) {
-                const float2 r = cs[(d0 + e) >> 1];
-                const double va = v0[e], vb = v0[e + 1], co = r.x, si = r.y;
-                v0[e] = (float)(va * co - vb * si);
-                v0[e + 1] = (float)(va * si + vb * co);
-            }
-            if (d1 + e < a.rot) {
-                const float2 r = cs[(d1 + e) >> 1];
-                const double va = v1[e], vb = v1[e + 1], co = r.x, si = r.y;
-                v1[e] = (float)(va * co - vb * si);
-                v1[e + 1] = (float)(va * si + vb * co);
-            }
-        }
+    for (int u = 0; u < kQHeads; ++u) {
+        const int h = min(h0 + u * a.by_heads.d, a.n_heads - 1);
+        v0[u] = *(const kq_f4*)(x + (size_t)h * HD + d0);
+        v1[u] = *(const kq_f4*)(x + (size_t)h * HD + d1);
     }
-    *(kq_f4*)(q + d0) = v0;
-    *(kq_f4*)(q + d1) = v1;
+#pragma unroll
+    for (int u = 0; u < kQHeads; ++u) {
+        const int h = h0 + u * a.by_heads.d;
+        if (h >= a.n_heads) break;
+        if (mode == kRotHalf) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const double va = v0[u][e], vb = v1[u][e], co = r[e].x, si = r[e].y;
+                v0[u][e] = (float)(va * co - vb * si);
+                v1[u][e] = (float)(va * si + vb * co);
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                kq_f4& v = e < 2 ? v0[u] : v1[u];
+                const double va = v[e % 2 * 2], vb = v[e % 2 * 2 + 1], co = r[e].x, si = r[e].y;
+                if (d0 + 2 * e < a.rot) {
+                    v[e % 2 * 2] = (float)(va * co - vb * si);
+                    v[e % 2 * 2 + 1] = (float)(va * si + vb * co);
+                }
+            }
+        }
+        *(kq_f4*)(q + (size_t)h * HD + d0) = v0[u];
+        *(kq_f4*)(q + (size_t)h * HD + d1) = v1[u];
+    }
 }
 
 // Grid: blocks_kv workgroups of K and V blocks (nblk a sequence and head), then q. kRotAny's q vectors, whose pairs lie
@@ -422,7 +432,7 @@ __global__ __launch_bounds__(256) void k_kvq_store_blocks(StoreArgs a, int mode,
     }
     const int lane = threadIdx.x & 63, hv = w * 4 + (threadIdx.x >> 6), row = a.by_heads(hv);
     if (row >= a.n_seq * a.n_tok) return;
-    const int h = hv - row * a.n_heads, seq = a.by_tok(row), start = kvq_start(a.d_pos, seq, a.pos_off, a.ctx);
+    const int h = hv - row * a.by_heads.d, seq = a.by_tok(row), start = kvq_start(a.d_pos, seq, a.pos_off, a.ctx);
     const int64_t p = (int64_t)start + (row - seq * a.n_tok);
     if (start < 0 || p >= a.ctx) return;
     const float* x = a.qkv + (int64_t)row * a.ldqkv + (size_t)h * HD;
@@ -633,7 +643,7 @@ extern "C" int orc_kvq_store(int type, const float* d_qkv, int ldqkv, int n_seq,
     if (rows > 0x7fffffff) return set_error(ORC_E_INVALID, "kvq_store: too many rows");
     const int64_t blocks = (rows * vecs + 3) / 4;
     if (n_tok < kStoreBlocks && blocks > 0xffffff00ll / 256) return set_error(ORC_E_INVALID, "kvq_store: too many rows");
-    const StoreArgs a{d_qkv, ldqkv, n_seq, n_tok, n_heads, n_kv, rope_layout, rot_dim, (const float2*)d_rope, rope_off,
+    StoreArgs a{d_qkv, ldqkv, n_seq, n_tok, n_heads, n_kv, rope_layout, rot_dim, (const float2*)d_rope, rope_off,
                       d_pos, pos_off, d_q, ldq, (uint8_t*)d_kc, (uint8_t*)d_vc, ctx, kvq_div((int)vecs), kvq_div(n_tok),
                       kvq_div(n_heads)};
     const hipStream_t st = resolve_stream(s);
@@ -651,7 +661,8 @@ extern "C" int orc_kvq_store(int type, const float* d_qkv, int ldqkv, int n_seq,
     else {
         const int mode = rope_layout == ORC_ROPE_PAIRS || !rot_dim ? kRotPairs : rot_dim == head_dim ? kRotHalf : kRotAny;
         const int nblk = (int)(((int64_t)n_tok + 2 * kKvBlock - 2) / kKvBlock);  // blocks that n_tok rows may touch
-        const int64_t kv = (int64_t)n_seq * 2 * n_kv * nblk, q = rows * n_heads;
+        if (mode != kRotAny) a.by_heads = kvq_div((n_heads + kQHeads - 1) / kQHeads);
+        const int64_t kv = (int64_t)n_seq * 2 * n_kv * nblk, q = rows * a.by_heads.d;
         const int64_t all = kv + (mode == kRotAny ? (q + 3) / 4 : (q * (head_dim / 8) + 255) / 256);
         if (all > 0xffffff00ll / 256) return set_error(ORC_E_INVALID, "kvq_store: too many rows");
         each([&](auto ty, auto hd) {
