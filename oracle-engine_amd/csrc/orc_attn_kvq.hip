@@ -1090,11 +1090,11 @@ struct KaPlan {
 
 static int ka_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 
-// Chunks of nb key blocks for `base` workgroups' worth of row tiles: at most `most` workgroups, and four blocks each or
-// more, all of a length but the last; one where `one` blocks are no more work than a second launch.
-static int ka_chunks(int64_t base, int nb, int64_t most, int one) {
+// Chunks of nb key blocks for `base` workgroups' worth of row tiles: at most `most` workgroups, and `least` blocks each
+// or more, all of a length but the last; one where `one` blocks are no more work than a second launch.
+static int ka_chunks(int64_t base, int nb, int64_t most, int one, int least) {
     if (nb <= one) return 1;
-    const int n = (int)std::max<int64_t>(1, std::min<int64_t>(most / base, (nb + 3) / 4));
+    const int n = (int)std::max<int64_t>(1, std::min<int64_t>(most / base, (nb + least - 1) / least));
     return ka_div(nb, ka_div(nb, n));
 }
 
@@ -1123,13 +1123,20 @@ static KaPlan ka_plan(int n_seq, int n_tok, int n_heads, int n_kv, int hd, int p
     // second adds no bandwidth but partial sums: 32000 tokens, 32/8 heads of 128, 8 bits: 23.9 us with 512, 19.3 with
     // 256; 16 sequences x 4 tokens of 4000, 28/4 heads: 33.6 and 27.7; but 512 tokens after 7500: 135 and 178).
     const int64_t base_o = (int64_t)n_seq * n_kv * p.tiles_o, fill = 512 / p.kg;
-    p.co = ka_chunks(base_o, p.shared ? nbo : nbp + nbo, p.m_o <= 32 ? 256 : fill, p.m_o <= 32 ? 12 : 4 * p.kg);
+    // Few blocks stay one chunk, for the merge is a launch: up to two for each wave (8 blocks, 8 bits: 8.3 us against 9.9;
+    // 12: 10.2 against 9.8; at 64 dims 12: 7.6 against 8.6) or three for each group of waves that share operands (9
+    // tokens at 300 and 500, 28/4 heads: 12.1 against 12.6, and 15.2 against 12.9). Beyond, two a chunk or more (5 tokens
+    // at 1000: 14.0 us with 4, 12.0 with 2).
+    p.co = ka_chunks(base_o, p.shared ? nbo : nbp + nbo, p.m_o <= 32 ? 256 : fill, p.m_o > 32 ? 3 * p.kg : hd == 64 ? 12 : 8, 2);
     if (p.shared) {
         p.tiles_p = ka_div(rows_p, p.m_p);
         const int64_t base_p = (int64_t)n_kv * p.tiles_p;
         // short prefix chunks share the card with the own jobs; beside long ones those are done in passing
         const bool lng = nbp * base_p >= 16 * fill;
-        p.cp = ka_chunks(base_p, nbp, lng ? fill : std::max<int64_t>(fill / 2, fill - base_o * p.co), 4);
+        // (2 blocks or more a chunk, 4 where the own jobs fill the card: 16 sequences after 1000 tokens, 28/4 heads of 128:
+        // 15.2 us with 4, 13.5 with 2; 64 after 500, 32/8 heads: 20.3 and 21.7)
+        p.cp = ka_chunks(base_p, nbp, lng ? fill : std::max<int64_t>(fill / 2, fill - base_o * p.co), 4,
+                         base_o * p.co >= fill ? 4 : 2);
     }
     return p;
 }
