@@ -275,6 +275,8 @@ LARGE = [
     (1, 1, 8, 2, 0, [5000], None, 5056),
     # own rows of several blocks a wave beside a prefix's tiles
     (17, 1, 8, 2, 1000, [37 * i for i in range(17)], None, 640), (4, 3, 28, 4, 200, [600, 331, -1, 63], None, 640),
+    # chunks by the hundred, of own rows and of a prefix
+    (1, 1, 8, 1, 0, [33000], None, 33024), (3, 1, 8, 1, 17000, [9000, 5, 8999], None, 9024), (5, 1, 8, 1, 70001, [40, 0, 7, 63, -1], None, 64),
     (100, 1, 16, 4, 12300, [3 * i for i in range(100)], None, 320), (25, 5, 16, 4, 12300, [12 * i for i in range(25)], None, 320),
 ]
 
@@ -508,6 +510,26 @@ def test_store_in_place_of_every_form(dev, T, layout, rot):
     y = b.store(qkv, T, H, rope, rot, layout, [9, 70], in_place=True)
     assert np.array_equal(y[:, :H * hd], q[:, :-4]) and np.array_equal(y[:, H * hd:], qkv[:, H * hd:])
     assert np.array_equal(a.k.read(np.uint8), b.k.read(np.uint8)) and np.array_equal(a.v.read(np.uint8), b.v.read(np.uint8))
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("H,layout,rot", [(5, orc.ROPE_HALF, None), (6, orc.ROPE_PAIRS, None), (7, orc.ROPE_PAIRS, 38),
+                                          (14, orc.ROPE_HALF, None), (3, orc.ROPE_HALF, 38)])
+def test_a_prompt_is_written_as_its_tokens_one_by_one(dev, hd, H, layout, rot):
+    rng = np.random.default_rng(H)
+    S, T, KV, ctx, rot = 2, 41, 1, 128, rot or hd
+    starts = np.array([3, 70])
+    qkv = rng.normal(0, 1, (S, T, (H + 2 * KV) * hd)).astype(np.float32)
+    rope = _table(dev, 0, ctx, rot, 1e4)
+    a, b, c = (Caches(dev, orc.KV_Q8, S, KV, ctx, hd) for _ in range(3))
+    q = a.store(qkv.reshape(S * T, -1), T, H, rope, rot, layout, starts)[:, :H * hd].reshape(S, T, -1)
+    y = b.store(qkv.reshape(S * T, -1), T, H, rope, rot, layout, starts, in_place=True)[:, :H * hd].reshape(S, T, -1)
+    assert np.array_equal(q, y)
+    for t in range(T):
+        one = c.store(np.ascontiguousarray(qkv[:, t]), 1, H, rope, rot, layout, starts + t)
+        assert np.array_equal(one[:, :H * hd], q[:, t])
+    for other in (b, c):
+        assert np.array_equal(a.k.read(np.uint8), other.k.read(np.uint8)) and np.array_equal(a.v.read(np.uint8), other.v.read(np.uint8))
 
 
 @pytest.mark.parametrize("ty", [orc.F16, orc.KV_Q8])
